@@ -1,0 +1,504 @@
+"""Policy-training operators: their plain forms, their exact values, and the calls a program makes of the kernels.
+
+score   log-probabilities of the chosen items of ragged sequences (reference model, behaviour policy, serving of single tokens)
+pair    a preference loss over (chosen, rejected) sequences with the gradient of the logits
+policy  a clipped policy loss with a KL term, with the gradient of the logits
+adamw   an AdamW step over many tensors at once, moments in 32 or in 8 bits
+"""
+import math
+
+import torch
+
+own = False
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+WIDTH = {"f32": 4, "f16": 2, "bf16": 2}
+BLOCK = 64                       # values of an 8-bit moment that share a scale; tensors start at multiples of it in the flat buffers
+BETA1, BETA2, EPS, LR, DECAY = 0.9, 0.95, 1e-8, 2e-5, 0.1
+
+
+# ---- the cases ------------------------------------------------------------------------------------------------------------------------
+
+def listed():
+    return [
+        # two pairs of short slates over the items of one small table: launch latency
+        dict(name="pair, short slates", op="pair", seqs=4, longest=12, vocab=1000, dtype="f32", kind="logistic", mean_length=False, spare=3),
+        # a mini-batch with a catalogue of odd size: every row starts at another alignment; squared loss of mean log-probabilities
+        dict(name="pair, odd catalogue", op="pair", seqs=12, longest=150, vocab=30011, dtype="bf16", kind="square", mean_length=True, spare=5),
+        # a full batch of preference training: twice the logits of a step are larger than every cache
+        dict(name="pair, full batch", op="pair", seqs=16, longest=700, vocab=100000, dtype="bf16", kind="logistic", mean_length=False, spare=0),
+        # an online update on a handful of sessions
+        dict(name="policy, few sessions", op="policy", seqs=5, longest=8, vocab=2000, dtype="f32", per_row=False, kl=0.0, reduction="sum", spare=0),
+        # half precision with a scaled loss, odd catalogue, KL to the reference policy
+        dict(name="policy, odd catalogue", op="policy", seqs=16, longest=120, vocab=50021, dtype="f16", per_row=True, kl=0.05, reduction="token_mean", spare=7),
+        # a full batch of policy training with one advantage a sequence
+        dict(name="policy, full batch", op="policy", seqs=32, longest=400, vocab=100000, dtype="bf16", per_row=False, kl=0.02, reduction="sequence_mean", spare=0),
+        # serving: one new token of each of 32 sessions is scored
+        dict(name="score, single tokens", op="score", seqs=32, longest=1, vocab=100000, dtype="bf16", mean_length=False, spare=0),
+        # the reference model's pass over a batch, 32-bit logits
+        dict(name="score, long sequences", op="score", seqs=6, longest=900, vocab=50000, dtype="f32", mean_length=False, spare=11),
+        # the dense parameters of a click tower 429 - 256 - 128 - 64 - 1, clipped
+        dict(name="adamw, click tower", op="adamw", tensors=14, total=153000, bits=32, grad="f32", clip=True, copy=False),
+        # a large model: a hundred tensors, clipped, with the half copy that the next forward pass reads
+        dict(name="adamw, large model", op="adamw", tensors=100, total=120000000, bits=32, grad="f32", clip=True, copy=True),
+        # moments in 8 bits, a middling model
+        dict(name="adamw 8 bits, middling", op="adamw", tensors=37, total=3000000, bits=8, grad="f32", clip=False, copy=False),
+        # moments in 8 bits, gradients in 16: what a large model keeps when memory is short
+        dict(name="adamw 8 bits, large model", op="adamw", tensors=200, total=200000000, bits=8, grad="bf16", clip=True, copy=True),
+    ]
+
+
+def _log_uniform(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(("score", "pair", "policy", "adamw"))
+    if op == "adamw":
+        total = _log_uniform(rng, 2000, 100000000)
+        return dict(op=op, tensors=rng.randint(1, 150), total=total, bits=rng.choice((8, 32)), grad=rng.choice(("f32", "bf16")), clip=rng.random() < 0.5, copy=rng.random() < 0.5)
+    dtype = rng.choice(("f32", "f16", "bf16"))
+    vocab = _log_uniform(rng, 200, 120000) | (1 if rng.random() < 0.5 else 0)
+    rows = _log_uniform(rng, 4, max(5, min(12000, 150000000 // vocab)))          # up to about 150 million logits, twice that where they are few
+    seqs = max(2, min(64, _log_uniform(rng, 2, max(3, rows // 2))) // 2 * 2)
+    c = dict(op=op, seqs=seqs, longest=max(1, (2 * rows) // seqs), vocab=vocab, dtype=dtype, spare=rng.choice((0, 0, 1, 6)))
+    if op == "policy":
+        c.update(per_row=rng.random() < 0.5, kl=rng.choice((0.0, 0.05)), reduction=rng.choice(("sum", "token_mean", "sequence_mean")))
+    else:
+        c.update(mean_length=rng.random() < 0.5)
+    if op == "pair":
+        c.update(kind=rng.choice(("logistic", "square")))
+    return c
+
+
+def _lengths(case):
+    """Ragged and the same for every seed: the longest first, then spread between 1 and the longest."""
+    n = case["longest"]
+    return [n if i == 0 else 1 + int((n - 1) * math.modf(i * 0.6180339887)[0]) for i in range(case["seqs"])]
+
+
+def _masked(case):
+    """Rows of each sequence that are no action: the first third of it; all of the fourth sequence where there are more than eight."""
+    return [n if i == 3 and case["seqs"] > 8 else n // 3 for i, n in enumerate(_lengths(case))]
+
+
+def _sizes(case):
+    """Ragged tensors that add up to about `total`: matrices of several sizes, and every third a vector."""
+    k = case["tensors"]
+    share = [(0.002 if i % 3 == 2 else 1.0 + 3.0 * math.modf(i * 0.6180339887)[0]) for i in range(k)]
+    return [max(1, int(case["total"] * s / sum(share))) for s in share]
+
+
+def _starts(sizes):
+    at, n = [], 0
+    for s in sizes:
+        at.append(n)
+        n += -(-s // BLOCK) * BLOCK
+    return at, n
+
+
+# ---- inputs ---------------------------------------------------------------------------------------------------------------------------
+
+def prepare(case, seed):
+    g = torch.Generator("cuda").manual_seed(seed)
+    return _prepare_adamw(case, g, seed) if case["op"] == "adamw" else _prepare_rows(case, g)
+
+
+def _prepare_rows(case, g):
+    dev, V, dtype = "cuda", case["vocab"], TYPES[case["dtype"]]
+    lengths, masked = _lengths(case), _masked(case)
+    live_rows, T = sum(lengths), sum(lengths) + case["spare"]
+    position = torch.cat([torch.arange(n) for n in lengths] + [torch.arange(case["spare"])])
+    first = torch.cat([torch.full((n,), m) for n, m in zip(lengths, masked)] + [torch.zeros(case["spare"], dtype=torch.int64)])
+    live = (position >= first).to(dev)
+    live[live_rows:] = False
+    targets = torch.randint(0, V, (T,), device=dev, generator=g)
+    logits = torch.empty(T, V, dtype=dtype, device=dev)
+    score = torch.empty(T, device=dev)
+    step = max(1, (1 << 27) // V)
+    for r in range(0, T, step):          # what a trained model answers: a spread of scores, the chosen item among the likely ones
+        z = torch.randn(min(step, T - r), V, device=dev, generator=g) * 2.0
+        z[:, :: 97] = -math.inf          # items that this request may not show
+        t = targets[r: r + step].unsqueeze(1)
+        z.scatter_(1, t, 3.0 + 2.0 * torch.randn(t.shape, device=dev, generator=g))
+        z = z.to(dtype)
+        logits[r: r + step] = z
+        score[r: r + step] = (z.gather(1, t).float() - torch.logsumexp(z.float(), 1, True)).squeeze(1)
+    dead = (~live).nonzero().squeeze(1)
+    logits[dead[::2]] = math.nan         # what stands at masked positions is nobody's answer
+    offs = torch.tensor([0] + lengths).cumsum(0)
+    s = dict(case=case, logits=logits, targets=torch.where(live, targets, -1).to(torch.int32), offs=offs.to(dev, torch.int32))
+    if case["op"] == "score":
+        return s
+    s["dlogits"] = torch.zeros(T, V, dtype=dtype, device=dev)
+    s["scale"] = 4096.0 if case["dtype"] == "f16" else 1.0       # gradients in fp16 are those of a scaled loss
+    N = case["seqs"]
+    noise = torch.randn(N, device=dev, generator=g)
+    if case["op"] == "pair":
+        lp = torch.where(live, score, 0.0).double()[:live_rows]
+        total = torch.zeros(N, dtype=torch.float64, device=dev).index_add_(0, _row_sequence(s["offs"], live_rows), lp)
+        if case["mean_length"]:
+            total = total / torch.tensor([max(1, n - m) for n, m in zip(lengths, masked)], device=dev)
+        s["ref"] = (total + noise * (1.0 if case["mean_length"] else 6.0)).float()
+        s["weights"] = torch.rand(N // 2, device=dev, generator=g) + 0.5
+        return s
+    d = torch.randn(T, device=dev, generator=g) * 0.15          # log ratio to the behaviour policy
+    for edge in (math.log1p(0.2), math.log1p(-0.2)):            # none within 1e-4 of a clipping border: either answer is right there
+        d = torch.where((d - edge).abs() < 1e-4, d + 3e-4, d)
+    s["old"] = score - d
+    s["ref"] = score + 0.3 * torch.randn(T, device=dev, generator=g) if case["kl"] else None
+    s["advantages"] = torch.randn(T, device=dev, generator=g) if case["per_row"] else noise
+    return s
+
+
+def _prepare_adamw(case, g, seed):
+    dev = "cuda"
+    sizes = _sizes(case)
+    at, n = _starts(sizes)
+    inside = torch.zeros(n, dtype=torch.bool, device=dev)
+    for a, k in zip(at, sizes):
+        inside[a: a + k] = True
+    spread = torch.exp(torch.randn(n, device=dev, generator=g))           # parameters differ in how large their gradients are
+    grad = inside * (1e-3 * spread * torch.randn(n, device=dev, generator=g))
+    m = inside * (3e-4 * spread * torch.randn(n, device=dev, generator=g))
+    r = inside * (1e-3 * spread * (0.5 + torch.rand(n, device=dev, generator=g)))      # root of the second moment
+    s = dict(case=case, sizes=sizes, at=at, n=n, p=inside * (0.05 * torch.randn(n, device=dev, generator=g)), grad=grad.to(TYPES[case["grad"]]),
+             decay=[0.0 if i % 3 == 2 else DECAY for i in range(len(sizes))], clip=0.5 * 2.7e-3 * math.sqrt(sum(sizes)) if case["clip"] else None,      # about half of the norm
+             copy=torch.zeros(n, dtype=torch.bfloat16, device=dev) if case["copy"] else None, seed=seed & 0xffff, step=7)
+    if case["bits"] == 32:
+        s["m"], s["v"] = m, r * r
+    else:
+        half = torch.full((n,), 0.5, device=dev)
+        s["m"], s["m_scale"] = _encode(m, half, 3, True)
+        s["r"], s["r_scale"] = _encode(r, half, 4, False)
+    if own:
+        from wide_deep_amd import optim
+        views = lambda flat: [flat[a: a + k] for a, k in zip(at, sizes)]
+        opt = optim.AdamW(views(s["p"]), views(s["grad"]), lr=LR, betas=(BETA1, BETA2), eps=EPS, weight_decay=s["decay"], max_norm=s["clip"],
+                          state_bits=case["bits"], copies=None if s["copy"] is None else views(s["copy"]), seed=s["seed"])
+        for name in ("m", "v") if case["bits"] == 32 else ("m", "m_scale", "r", "r_scale"):
+            getattr(opt, name).copy_(s.pop(name))
+        opt.set_step(s["step"])
+        s["opt"] = opt
+    return s
+
+
+def _row_sequence(offs, rows):
+    return torch.bucketize(torch.arange(rows, device=offs.device), offs[1:].long(), right=True)
+
+
+# ---- one pass -------------------------------------------------------------------------------------------------------------------------
+
+def run(s):
+    return {"score": _score, "pair": _pair, "policy": _policy, "adamw": _adamw}[s["case"]["op"]](s)
+
+
+def _plain_rows(s):
+    """Softmax of each row, log-probability of its target (0 at masked rows), which rows count, and their sequence."""
+    live = s["targets"] >= 0
+    t = s["targets"].clamp(min=0).long().unsqueeze(1)
+    x = s["logits"].float()
+    x = x - x.amax(1, keepdim=True)
+    picked = x.gather(1, t).squeeze(1)
+    x = x.exp_()
+    total = x.sum(1)
+    rows = s["targets"].numel()
+    seq = _row_sequence(s["offs"], rows)
+    live = live & (seq < s["offs"].numel() - 1)
+    return x, total, torch.where(live, picked - total.log(), 0.0), live, seq.clamp(max=s["offs"].numel() - 2), t
+
+
+def _plain_sequences(s, lp, live, seq):
+    n = s["offs"].numel() - 1
+    total = torch.zeros(n, dtype=torch.float64, device=lp.device).index_add_(0, seq, lp.double())
+    count = torch.zeros(n, dtype=torch.float64, device=lp.device).index_add_(0, seq, live.double())
+    return total, count
+
+
+def _plain_gradient(s, x, total, live, t, coef):
+    """coef (1[target] - softmax), 0 at masked rows, rows behind the last sequence as they were."""
+    coef = torch.where(live, coef, 0.0)
+    x = x.mul_((-coef / total).unsqueeze(1))
+    x.scatter_add_(1, t, coef.unsqueeze(1))
+    x[~live] = 0.0
+    end = s["targets"].numel() - s["case"]["spare"]
+    s["dlogits"][:end] = x[:end].to(s["dlogits"].dtype)
+    return s["dlogits"]
+
+
+def _score(s):
+    c = s["case"]
+    if own:
+        from wide_deep_amd import policy
+        r = policy.sequence_logp(s["logits"], s["targets"], s["offs"], length_norm=c["mean_length"])
+        return {"token": r.token_logp, "sequence": r.seq_logp}
+    x, total, lp, live, seq, _ = _plain_rows(s)
+    sums, count = _plain_sequences(s, lp, live, seq)
+    return {"token": lp, "sequence": (sums / count.clamp(min=1) if c["mean_length"] else sums).float()}
+
+
+PAIR_BETA, PAIR_SMOOTH, PAIR_MARGIN = 0.1, 0.05, 0.25
+
+
+def _pair(s):
+    c = s["case"]
+    if own:
+        from wide_deep_amd import policy
+        smooth, margin = (PAIR_SMOOTH, PAIR_MARGIN) if c["kind"] == "logistic" else (0.0, 0.0)
+        r = policy.preference_loss(s["logits"], s["targets"], s["offs"], ref_logp=s["ref"], weights=s["weights"], kind=c["kind"], beta=PAIR_BETA,
+                                   margin=margin, label_smoothing=smooth, length_norm=c["mean_length"], reduction="mean",
+                                   grad_scale=s["scale"], dlogits=s["dlogits"])
+        return {"loss": r.loss, "pair_loss": r.pair_loss, "difference": r.difference, "sequence": r.seq_logp, "dlogits": r.dlogits}
+    x, total, lp, live, seq, t = _plain_rows(s)
+    sums, count = _plain_sequences(s, lp, live, seq)
+    norm = count.clamp(min=1) if c["mean_length"] else torch.ones_like(count)
+    logp = sums / norm
+    d = (logp - s["ref"].double()).view(-1, 2)
+    d = d[:, 0] - d[:, 1]
+    w = s["weights"].double()
+    if c["kind"] == "logistic":
+        h = PAIR_BETA * d - PAIR_MARGIN
+        pair = -(1 - PAIR_SMOOTH) * torch.nn.functional.logsigmoid(h) - PAIR_SMOOTH * torch.nn.functional.logsigmoid(-h)
+        slope = PAIR_BETA * (torch.sigmoid(h) - (1 - PAIR_SMOOTH))
+    else:
+        h = d - 1 / (2 * PAIR_BETA)
+        pair, slope = h * h, 2 * h
+    slope = slope * w / w.numel()
+    coef = (torch.stack((slope, -slope), 1).view(-1) / norm * s["scale"])[seq].float()
+    grad = _plain_gradient(s, x, total, live, t, coef)
+    return {"loss": ((pair * w).sum() / w.numel()).float(), "pair_loss": pair.float(), "difference": d.float(), "sequence": logp.float(), "dlogits": grad}
+
+
+def _policy(s):
+    c = s["case"]
+    if own:
+        from wide_deep_amd import policy
+        r = policy.policy_loss(s["logits"], s["targets"], s["offs"], s["old"], s["advantages"], ref_logp=s["ref"], clip=(0.2, 0.2), kl_coef=c["kl"],
+                               reduction=c["reduction"], grad_scale=s["scale"], dlogits=s["dlogits"])
+        return {"loss": r.loss, "kl": r.kl, "clipped": r.clipped, "token": r.token_logp, "dlogits": r.dlogits}
+    x, total, lp, live, seq, t = _plain_rows(s)
+    _, count = _plain_sequences(s, lp, live, seq)
+    w = {"sum": torch.ones_like(lp), "token_mean": torch.ones_like(lp) / count.sum().clamp(min=1).float(),
+         "sequence_mean": (1 / (count.clamp(min=1) * (count > 0).sum().clamp(min=1))).float()[seq]}[c["reduction"]]
+    w = torch.where(live, w, 0.0)
+    adv = s["advantages"] if c["per_row"] else s["advantages"][seq]
+    ratio = torch.exp(torch.where(live, lp - s["old"], 0.0))
+    free, held = ratio * adv, ratio.clamp(0.8, 1.2) * adv
+    gone = free > held
+    loss, slope, kl = -torch.minimum(free, held), torch.where(gone, 0.0, -free), torch.zeros_like(lp)
+    if c["kl"]:
+        q = torch.where(live, s["ref"] - lp, 0.0)
+        kl = torch.expm1(q) - q
+        loss, slope = loss + c["kl"] * kl, slope - c["kl"] * torch.expm1(q)
+    grad = _plain_gradient(s, x, total, live, t, slope * w * s["scale"])
+    return {"loss": (loss * w).double().sum().float(), "kl": (kl * w).double().sum().float(), "clipped": ((gone & live) * w).double().sum().float(),
+            "token": lp, "dlogits": grad}
+
+
+def _encode(x, dither, mantissa, signed):
+    """Codes and scale bytes of an 8-bit moment: 4 exponent bits, `mantissa` bits, a power-of-two scale for each BLOCK values; `dither` in [0, 1)
+    is what rounds up (0.5: to nearest).  The scale puts the block's largest value into the largest binade."""
+    top = x.abs().view(-1, BLOCK).amax(1)
+    scale = (top.view(torch.int32) >> 23).clamp(min=27)
+    y = (x.abs().view(-1, BLOCK) * torch.exp2(142.0 - scale).unsqueeze(1)).view(-1)
+    # the top binade of y is [2^15, 2^16); values under 2 (the lowest one) keep their absolute step
+    low = torch.floor(y * 2.0 ** (mantissa - 1) + dither).to(torch.int32)
+    high = ((y.view(torch.int32) + (dither * 2 ** (23 - mantissa)).to(torch.int32)) >> (23 - mantissa)) - (127 << mantissa)
+    code = torch.where(y < 2.0, low, high).clamp(max=16 * 2 ** mantissa - 1)
+    if signed:
+        code = code | (torch.signbit(x).to(torch.int32) << 7)
+    return code.to(torch.uint8), scale.to(torch.uint8)
+
+
+def _decode(code, scale, mantissa, signed):
+    c = code.to(torch.int32)
+    k = c & 127 if signed else c
+    high = ((k + (127 << mantissa)) << (23 - mantissa)).view(torch.float32)
+    y = torch.where(k < 2 ** mantissa, k * 2.0 ** (1 - mantissa), high)
+    y = (y.view(-1, BLOCK) * torch.exp2(scale.float() - 142.0).unsqueeze(1)).view(-1)
+    return torch.where(c >= 128, -y, y) if signed else y
+
+
+def _dither(n, seed, step, device):
+    """Two numbers in [0, 1) with 16 bits for each index: a hash of (index, step, seed)."""
+    i = torch.arange(n, device=device)
+    word = 0xFFFFFFFF
+    h = (((i & word) ^ seed) + step * 0x9E3779B1 + (i >> 32) * 0xBB67AE85) & word
+    h = ((h ^ (h >> 16)) * 0xBB67AE85) & word
+    h = ((h ^ (h >> 15)) * 0x6A09E667) & word
+    h = h ^ (h >> 16)
+    return (h >> 16).float() / 65536, (h & 0xFFFF).float() / 65536
+
+
+def _adamw(s):
+    c = s["case"]
+    if own:
+        opt = s["opt"]
+        opt.step()
+        out = {"p": s["p"], "copy": s["copy"], "norm": opt.grad_norm if c["clip"] else None}
+        out["m"], out["v"] = (opt.m, opt.v) if c["bits"] == 32 else opt.moments()
+        return out
+    s["step"] += 1
+    t, g, norm = s["step"], s["grad"].float(), None
+    if c["clip"]:
+        norm = g.double().square().sum().sqrt()
+        g = g * (s["clip"] / norm.clamp(min=s["clip"])).float()
+        norm = norm.float()
+    sizes = torch.tensor([b - a for a, b in zip(s["at"], s["at"][1:] + [s["n"]])], device=g.device)
+    decay = torch.repeat_interleave(torch.tensor(s["decay"], device=g.device), sizes, output_size=s["n"])
+    if c["bits"] == 32:
+        m, v = s["m"], s["v"]
+    else:
+        m, r = _decode(s["m"], s["m_scale"], 3, True), _decode(s["r"], s["r_scale"], 4, False)
+        v = r * r
+    m = BETA1 * m + (1 - BETA1) * g
+    v = BETA2 * v + (1 - BETA2) * g * g
+    s["p"] -= LR * (m / (1 - BETA1 ** t) / (torch.sqrt(v / (1 - BETA2 ** t)) + EPS) + decay * s["p"])
+    if c["copy"]:
+        s["copy"].copy_(s["p"])
+    out = {"p": s["p"], "copy": s["copy"], "norm": norm}
+    if c["bits"] == 32:
+        s["m"], s["v"] = out["m"], out["v"] = m, v
+    else:
+        dm, dr = _dither(s["n"], s["seed"], t, g.device)
+        s["m"], s["m_scale"] = _encode(m, dm, 3, True)
+        s["r"], s["r_scale"] = _encode(torch.sqrt(v), dr, 4, False)
+        out["m"], out["v"] = _decode(s["m"], s["m_scale"], 3, True).bfloat16(), _decode(s["r"], s["r_scale"], 4, False).bfloat16()
+    return out
+
+
+# ---- what a pass cannot do without ----------------------------------------------------------------------------------------------------
+
+def work(case):
+    if case["op"] == "adamw":
+        n, gb = sum(_sizes(case)), WIDTH[case["grad"]]
+        moments = 16 if case["bits"] == 32 else 4 + 4.0 / BLOCK + 4         # 8 bits: codes and scales read and written, the values returned
+        return {"bytes": n * (8 + gb + moments + (2 if case["copy"] else 0)), "flops": 15 * n}
+    rows = sum(_lengths(case))
+    live = rows - sum(_masked(case))
+    size = WIDTH[case["dtype"]] * case["vocab"]
+    if case["op"] == "score":
+        return {"bytes": live * size + 12 * rows, "flops": 5 * live * case["vocab"]}
+    return {"bytes": (live + rows) * size + 20 * rows, "flops": 9 * live * case["vocab"]}
+
+
+# ---- exact values ---------------------------------------------------------------------------------------------------------------------
+
+def exact(case, seed):
+    """The definitions in 64 bits, a row or a tensor at a time."""
+    global own
+    was, own = own, False
+    s = prepare(case, seed)
+    own = was
+    return _exact_adamw(s) if case["op"] == "adamw" else _exact_rows(s)
+
+
+def _exact_rows(s):
+    c, dev = s["case"], s["logits"].device
+    offs, targets = s["offs"].tolist(), s["targets"].tolist()
+    T, N, V = len(targets), c["seqs"], c["vocab"]
+    alive = [[r for r in range(offs[n], offs[n + 1]) if targets[r] >= 0] for n in range(N)]
+    flat = [r for rows in alive for r in rows]
+    index = torch.tensor(flat, dtype=torch.int64, device=dev)
+    chosen = s["targets"][index].long()
+    lse = torch.zeros(T, dtype=torch.float64, device=dev)
+    token = torch.zeros(T, dtype=torch.float64, device=dev)
+    step = max(1, (1 << 27) // V)
+    for a in range(0, len(flat), step):
+        at = index[a: a + step]
+        z = s["logits"][at].double()
+        lse[at] = torch.logsumexp(z, 1)
+        token[at] = z[torch.arange(at.numel(), device=dev), chosen[a: a + step]] - lse[at]
+    sums = [token[rows].sum() if rows else torch.zeros((), dtype=torch.float64, device=dev) for rows in alive]
+    norm = [max(1, len(rows)) if c.get("mean_length") else 1 for rows in alive]
+    sequence = torch.stack([a / b for a, b in zip(sums, norm)])
+    if c["op"] == "score":
+        return {"token": token, "sequence": sequence}
+    coef = torch.zeros(T, dtype=torch.float64, device=dev)
+    if c["op"] == "pair":
+        ref, w = s["ref"].double(), s["weights"].double()
+        d = sequence[0::2] - ref[0::2] - sequence[1::2] + ref[1::2]
+        if c["kind"] == "logistic":
+            h = PAIR_BETA * d - PAIR_MARGIN
+            each = (1 - PAIR_SMOOTH) * torch.log1p(torch.exp(-h)) + PAIR_SMOOTH * torch.log1p(torch.exp(h))
+            slope = -PAIR_BETA * ((1 - PAIR_SMOOTH) / (1 + torch.exp(h)) - PAIR_SMOOTH / (1 + torch.exp(-h)))
+        else:
+            each, slope = (d - 0.5 / PAIR_BETA) ** 2, 2 * d - 1 / PAIR_BETA
+        for n in range(N):
+            coef[alive[n]] = (1 - 2 * (n % 2)) * slope[n // 2] * w[n // 2] / (N // 2) / norm[n]
+        out = {"loss": (each * w).mean(), "pair_loss": each, "difference": d, "sequence": sequence}
+    else:
+        old, adv = s["old"].double(), s["advantages"].double()
+        full = sum(1 for rows in alive if rows)
+        out = {"loss": 0.0, "kl": 0.0, "clipped": 0.0, "token": token}
+        for n, rows in enumerate(alive):
+            if not rows:
+                continue
+            w = {"sum": 1.0, "token_mean": 1.0 / max(1, len(flat)), "sequence_mean": 1.0 / (len(rows) * max(1, full))}[c["reduction"]]
+            a = adv[rows] if c["per_row"] else adv[n]
+            rho = torch.exp(token[rows] - old[rows])
+            bounded = torch.where(rho > 1.2, 1.2, torch.where(rho < 0.8, 0.8, rho))
+            stopped = rho * a > bounded * a
+            loss, slope = -torch.where(stopped, bounded, rho) * a, torch.where(stopped, 0.0, -rho * a)
+            if c["kl"]:
+                q = s["ref"].double()[rows] - token[rows]
+                k = torch.exp(q) - q - 1
+                loss, slope = loss + c["kl"] * k, slope + c["kl"] * (1 - torch.exp(q))
+                out["kl"] = out["kl"] + w * k.sum()
+            out["loss"] = out["loss"] + w * loss.sum()
+            out["clipped"] = out["clipped"] + w * stopped.double().sum()
+            coef[rows] = w * slope
+        # numbers of a case without a KL term or a live row
+        out.update({k: torch.as_tensor(v, dtype=torch.float64, device=dev) for k, v in out.items()})
+    grad = torch.zeros(T, V, dtype=torch.float64, device=dev)
+    for a in range(0, len(flat), step):
+        at = index[a: a + step]
+        part = -torch.exp(s["logits"][at].double() - lse[at].unsqueeze(1))
+        part[torch.arange(at.numel(), device=dev), chosen[a: a + step]] += 1
+        grad[at] = part * (coef[at] * s["scale"]).unsqueeze(1)
+    return {**out, "dlogits": grad}
+
+
+def _exact_values(mantissa):
+    """What the codes 0 .. stand for with a scale of one, ascending."""
+    low = [f * 2.0 ** (1 - mantissa) for f in range(2 ** mantissa)]
+    return low + [2.0 ** e * (1 + f / 2 ** mantissa) for e in range(1, 16) for f in range(2 ** mantissa)]
+
+
+def _exact_round(x, dither, mantissa, values):
+    """The neighbour of x below, or the one above where the dither says so, by a search among the values that a block can hold."""
+    blocks = x.abs().view(-1, BLOCK)
+    exponent = torch.floor(torch.log2(blocks.amax(1).clamp(min=2.0 ** -100)))
+    exponent = torch.where(torch.exp2(exponent) > blocks.amax(1).clamp(min=2.0 ** -100), exponent - 1, exponent)
+    unit = torch.exp2(exponent - 15).unsqueeze(1)
+    y = (blocks / unit).view(-1)
+    below = (torch.searchsorted(values, y, right=True) - 1).clamp(max=values.numel() - 1)
+    above = (below + 1).clamp(max=values.numel() - 1)
+    gap = (values[above] - values[below]).clamp(min=1e-300)
+    up = (y - values[below]) / gap + dither >= 1
+    picked = torch.where(up, values[above], values[below])
+    return (picked.view(-1, BLOCK) * unit).view(-1) * torch.where(x < 0, -1.0, 1.0)
+
+
+def _exact_adamw(s):
+    c = s["case"]
+    t = s["step"] + 1
+    g = s["grad"].double()
+    norm = torch.sqrt((g * g).sum())
+    if c["clip"]:
+        g = g * min(1.0, s["clip"] / float(norm))
+    if c["bits"] == 32:
+        m, v = s["m"].double(), s["v"].double()
+    else:
+        m, v = _decode(s["m"], s["m_scale"], 3, True).double(), _decode(s["r"], s["r_scale"], 4, False).double() ** 2
+    m, v = m * BETA1 + g * (1 - BETA1), v * BETA2 + g * g * (1 - BETA2)
+    p = s["p"].double()
+    for a, k, decay in zip(s["at"], s["sizes"], s["decay"]):
+        part = slice(a, a + k)
+        p[part] = p[part] * (1 - LR * decay) - LR * (m[part] / (1 - BETA1 ** t)) / (torch.sqrt(v[part] / (1 - BETA2 ** t)) + EPS)
+    out = {"p": p, "copy": p if c["copy"] else None, "norm": norm if c["clip"] else None, "m": m, "v": v}
+    if c["bits"] == 8:
+        dm, dr = _dither(s["n"], s["seed"], t, g.device)
+        out["m"] = _exact_round(m, dm.double(), 3, torch.tensor(_exact_values(3), dtype=torch.float64, device=g.device))
+        out["v"] = _exact_round(torch.sqrt(v), dr.double(), 4, torch.tensor(_exact_values(4), dtype=torch.float64, device=g.device))
+    return out
