@@ -273,8 +273,8 @@ def _policy(s):
     c = s["case"]
     if own:
         from wide_deep_amd import policy
-        r = policy.policy_loss(s["logits"], s["targets"], s["offs"], s["old"], s["advantages"], ref_logp=s["ref"], clip=(0.2, 0.2), kl_coef=c["kl"],
-                               reduction=c["reduction"], grad_scale=s["scale"], dlogits=s["dlogits"])
+        r = policy.policy_loss(s["logits"], s["targets"], s["offs"], s["old"], s["advantages"], ref_logp=s["ref"], per_row=c["per_row"], clip=(0.2, 0.2),
+                               kl_coef=c["kl"], reduction=c["reduction"], grad_scale=s["scale"], dlogits=s["dlogits"])
         return {"loss": r.loss, "kl": r.kl, "clipped": r.clipped, "token": r.token_logp, "dlogits": r.dlogits}
     x, total, lp, live, seq, t = _plain_rows(s)
     _, count = _plain_sequences(s, lp, live, seq)
