@@ -862,6 +862,126 @@ int wd_small_tables_apply(float *emb, float *emb_accum, float *wide_wzn, const w
                           const int32_t *small_idx, int32_t nsmall, int32_t max_rows, int32_t max_dim, const float *gsum,
                           float lr_emb, float lr_wide, float l1, float l2, int32_t rec_stride, wd_stream_t stream);
 
+/* ---- heads of a policy over items (no counterpart in the reference, whose only head is the sigmoid CE of wd_bce_sum_fwd_bwd) ----
+ * Logits z[r][v] of `rows` positions over `vocab` items, row stride ld (elements), and the chosen item targets[r] of each; a target
+ * outside [0, vocab) (-1) marks a position that is no action of the policy (prompt, padding): its logits are never read -- they may
+ * hold NaN --, its log-probability is 0 and its gradient 0.  Sequences are a CSR over the rows: sequence n = rows [seq_offs[n],
+ * seq_offs[n + 1]), ascending; rows in front of the first and behind the last sequence belong to nobody: token_logp there is 0, a
+ * gradient buffer is left as it was (zero_tail != 0: zeroed).  An item with logit -inf has probability 0.  Rows may start at any
+ * multiple of the element size.  dlogits may be the logits' own buffer.  ws: wd_policy_workspace_floats(rows) floats, 8-byte aligned,
+ * for one call at a time (negative: the arguments are refused).  At most 2^30 rows and items, 2^29 sequences.  All launches go to
+ * `stream`; nothing is read back. */
+#define WD_T_F32 0
+#define WD_T_F16 1
+#define WD_T_BF16 2
+typedef struct wd_seq_rows {
+  const void *logits;
+  int64_t ld, rows, vocab;
+  const int32_t *targets;    /* [rows] */
+  const int32_t *seq_offs;   /* [nseq + 1] */
+  int64_t nseq;
+  int32_t dtype;             /* WD_T_* of logits and gradient */
+  int32_t pad_;
+} wd_seq_rows_t;
+int64_t wd_policy_workspace_floats(const wd_seq_rows_t *rows);
+/* token_logp[r] = log softmax(z[r])[targets[r]]; seq_logp[n] = their sum over sequence n (length_norm: their mean over the actions
+ * of n; 0 without any).  Sums in 64 bits. */
+int wd_seq_logp(const wd_seq_rows_t *rows, int32_t length_norm, float *token_logp, float *seq_logp, float *ws, wd_stream_t stream);
+
+/* Preference loss: pair i = sequences 2i (chosen) and 2i + 1 (rejected), LP[n] as wd_seq_logp,
+ *   d = (LP[2i] - ref[2i]) - (LP[2i + 1] - ref[2i + 1])
+ *   LOGISTIC  h = beta d - margin;  pair_loss = -(1 - eps) log sigma(h) - eps log sigma(-h)
+ *   SQUARE    pair_loss = (d - 1 / (2 beta))^2          (no margin, no smoothing)
+ *   loss = scale sum_i weights[i] pair_loss[i]
+ * and dlogits = grad_scale dloss/dlogits (NULL: the loss alone). */
+#define WD_PREF_LOGISTIC 0
+#define WD_PREF_SQUARE 1
+typedef struct wd_pref {
+  const float *ref_logp;     /* [nseq], NULL: 0 */
+  const float *weights;      /* [nseq / 2], NULL: 1 */
+  float *loss;               /* [1] */
+  float *pair_loss;          /* [nseq / 2] */
+  float *difference;         /* [nseq / 2]: d */
+  float *seq_logp;           /* [nseq] */
+  float *token_logp;         /* [rows] */
+  void *dlogits;
+  int64_t ld_dlogits;
+  float beta, margin, label_smoothing, scale, grad_scale;
+  int32_t kind, length_norm, zero_tail;
+} wd_pref_t;
+int wd_pref_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_pref_t *opts, float *ws, wd_stream_t stream);
+
+/* Clipped policy loss: rho = e^(lp - old_logp[r]), A the advantage of the row or of its sequence,
+ *   l = -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef k,   k = e^(ref - lp) - (ref - lp) - 1  (ref_logp NULL: 0)
+ *   loss = sum_r w l;  w = 1 | 1 / actions | 1 / (sequences with an action x actions of the row's sequence)
+ * sums[0..2] = loss, sum w k, sum w [the clipped side was taken]; dlogits = grad_scale dloss/dlogits (NULL: the loss alone). */
+#define WD_POLICY_SUM 0
+#define WD_POLICY_TOKEN_MEAN 1
+#define WD_POLICY_SEQUENCE_MEAN 2
+typedef struct wd_policy {
+  const float *old_logp;     /* [rows] */
+  const float *ref_logp;     /* [rows] or NULL */
+  const float *advantages;   /* [rows] or [nseq] */
+  float *sums;               /* [3] */
+  float *token_logp;         /* [rows] */
+  void *dlogits;
+  int64_t ld_dlogits;
+  float clip_low, clip_high, kl_coef, grad_scale;
+  int32_t adv_per_row, reduction, zero_tail, pad_;
+} wd_policy_t;
+int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy_t *opts, float *ws, wd_stream_t stream);
+
+/* ---- AdamW over many tensors at once (beside wd_opt_dense: decoupled decay per tensor, clipping by the global norm, moments in 32
+ * or in 8 bits, a half copy of the parameters) ----
+ *   G = sqrt(sum g^2) over all tensors, g' = g max_norm / max(G, max_norm)            (max_norm <= 0: g' = g, G is not computed)
+ *   m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;  p -= lr (m / (1 - b1^t) / (sqrt(v / (1 - b2^t)) + eps) + decay p)
+ * With clipping, a step whose G is not finite changes nothing and is counted in wd_adamw_state_t.skipped.
+ * Moments live in flat buffers, tensor k from element tensors[k].start on (a multiple of WD_ADAMW_BLOCK; buffers as long as the
+ * padded sum).  bits 32: m, v float.  bits 8: m one byte of sign, 4 exponent and 3 mantissa bits, r = sqrt(v) one byte of 4 exponent
+ * and 4 mantissa bits; every block of WD_ADAMW_BLOCK values has one scale byte s, the (biased) binary exponent of its largest
+ * value, at least 27: value = code value x 2^(s - 142), code value of (e, f): (1 + f / 2^M) 2^e, e = 0: f 2^(1 - M).  A block with a value
+ * that is not finite has s = 255 and reads as NaN.  Values are rounded up with the probability of their fraction, by 16 bits for
+ * each moment from a hash of (flat index, step, seed): a second moment whose step is below half a code would otherwise never move. */
+#define WD_ADAMW_BLOCK 64
+#define WD_ADAMW_CHUNK 4096   /* elements of one entry of `chunks` */
+typedef struct wd_adamw_tensor {
+  float *p;
+  const void *g;
+  void *copy;                /* half copy of p written by the step, or NULL */
+  int64_t n, start;
+  float decay;
+  int32_t pad_;
+} wd_adamw_tensor_t;
+typedef struct wd_adamw_state {   /* device; written by wd_adamw_set_step, advanced by every wd_adamw_step that is not skipped */
+  int64_t step;              /* steps done */
+  int32_t skipped, ticket;
+  float corr1, corr2;        /* 1 / (1 - b1^(step + 1)), 1 / sqrt(1 - b2^(step + 1)) */
+  float norm, pad_;          /* G of the last step with clipping */
+} wd_adamw_state_t;
+typedef struct wd_adamw {
+  const wd_adamw_tensor_t *tensors;   /* device */
+  const int32_t *chunks;     /* device [nchunks][2]: tensor, chunk of it */
+  int64_t nchunks;
+  void *m, *v;               /* v: r's codes with 8 bits */
+  uint8_t *m_scale, *r_scale;
+  wd_adamw_state_t *state;
+  double *partials;          /* [WD_ADAMW_PARTIALS], clipping only */
+  const float *lr_dev;       /* device [1]: overrides lr (a captured step whose rate moves) */
+  double beta1, beta2;
+  float lr, eps, max_norm;
+  uint32_t seed;
+  int32_t bits, grad_dtype, copy_dtype, pad_;
+} wd_adamw_t;
+#define WD_ADAMW_PARTIALS 1024
+int wd_adamw_step(const wd_adamw_t *opts, wd_stream_t stream);
+int wd_adamw_set_step(wd_adamw_state_t *state, int64_t step, double beta1, double beta2, wd_stream_t stream);
+/* 8-bit moments <-> numbers, n values (a multiple of WD_ADAMW_BLOCK) from the start of the flat buffers; unpack: m and r as bf16 or
+ * fp32 (bf16 holds every value exactly), pack: to nearest from fp32 m and r. */
+int wd_adamw_unpack(const uint8_t *m, const uint8_t *m_scale, const uint8_t *r, const uint8_t *r_scale, int64_t n, void *out_m,
+                    void *out_r, int32_t out_dtype, wd_stream_t stream);
+int wd_adamw_pack(const float *in_m, const float *in_r, int64_t n, uint8_t *m, uint8_t *m_scale, uint8_t *r, uint8_t *r_scale,
+                  wd_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -260,12 +260,20 @@ _PROTOS = {
     "wd_counter_tick": [P, P],
     "wd_mlp_finalize": [P, I32, P, I64, I64, P, P, P, P, F32, P, I64, I64, P],
     "wd_adagrad_dense": [P, P, P, I64, F32, P],
+    "wd_policy_workspace_floats": [P],
+    "wd_seq_logp": [P, I32, P, P, P, P],
+    "wd_pref_loss_fwd_bwd": [P, P, P, P],
+    "wd_policy_loss_fwd_bwd": [P, P, P, P],
+    "wd_adamw_step": [P, P],
+    "wd_adamw_set_step": [P, I64, ctypes.c_double, ctypes.c_double, P],
+    "wd_adamw_unpack": [P, P, P, P, I64, P, P, I32, P],
+    "wd_adamw_pack": [P, P, I64, P, P, P, P, P],
     "wd_fill_f32": [P, F32, I64, P],
     "wd_diag_gather64": [P, P, I64, I32, P, P],
     "wd_diag_gather_modes": [P, I64, P, I64, I32, P, P],
     "wd_diag_access": [P, P, P, I32, P, I64, I32, I32, P, P],
 }
-_RESTYPES = {"wd_build_stamp": ctypes.c_char_p, "wd_prefetch_onehot_blocks": I64, "wd_feat_offsets_workspace_bytes": I64, "wd_sort_workspace_bytes": SZ, "wd_logits_head_blocks": I64, "wd_tower_chain_lds_bytes": I64, "wd_tower_chain_windows_lds_bytes": I64, "wd_tower_chain_blocks": I64, "wd_bucket_max": I32, "wd_bucket_chunks": I32, "wd_route_chunks": I32, "wd_small_tables_ws_floats": I64}
+_RESTYPES = {"wd_build_stamp": ctypes.c_char_p, "wd_prefetch_onehot_blocks": I64, "wd_feat_offsets_workspace_bytes": I64, "wd_sort_workspace_bytes": SZ, "wd_logits_head_blocks": I64, "wd_tower_chain_lds_bytes": I64, "wd_tower_chain_windows_lds_bytes": I64, "wd_tower_chain_blocks": I64, "wd_bucket_max": I32, "wd_bucket_chunks": I32, "wd_route_chunks": I32, "wd_small_tables_ws_floats": I64, "wd_policy_workspace_floats": I64}
 
 EXPORTED_SYMBOLS = sorted(list(_PROTOS) + ["wd_last_error"])
 

@@ -1,0 +1,729 @@
+// wide_deep_amd/csrc/policy_loss.hip -- heads of a policy over items: log-probabilities of the chosen items of ragged sequences,
+// a preference loss over pairs of sequences and a clipped policy loss with a KL term, each with the gradient of the logits.
+//
+// Mathematics (rows r of logits z[r, 0..V), chosen item t[r], sequences = CSR over rows):
+//   m = max_v z_v,  s = sum_v e^(z_v - m)                 one pass, running maximum and sum
+//   lp = (z_t - m) - ln s                                 (not z_t - lse: the difference keeps its low bits where |m| is large)
+//   dlp/dz_v = [v = t] - e^(z_v - m) / s,  dz_v = c * dlp/dz_v   with c = dloss/dlp of the row
+// Everything a row needs from other rows is a handful of numbers, so the kernels are passes over rows and HBM bounds them.
+#include "common.h"
+
+namespace {
+
+using namespace wd;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLowest = -3.402823466e38f;
+
+// ---- element types: one 16-byte word <-> floats.  Sums and statistics are fp32; gradients are rounded once, to nearest even.
+template <int DT> struct Elem;
+template <> struct Elem<WD_T_F32> {
+  typedef float type;
+  static constexpr int W = 4;
+  static __device__ __forceinline__ void unpack(const u32x4 &w, float *x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+  }
+  static __device__ __forceinline__ u32x4 pack(const float *x) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(x[i]);
+    return w;
+  }
+  static __device__ __forceinline__ float to_float(float v) { return v; }
+  static __device__ __forceinline__ float from_float(float v) { return v; }
+};
+template <> struct Elem<WD_T_BF16> {
+  typedef uint16_t type;
+  static constexpr int W = 8;
+  static __device__ __forceinline__ void unpack(const u32x4 &w, float *x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ u32x4 pack(const float *x) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x2 p = {x[2 * i], x[2 * i + 1]};
+      w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2));
+    }
+    return w;
+  }
+  static __device__ __forceinline__ float to_float(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+  static __device__ __forceinline__ uint16_t from_float(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
+};
+template <> struct Elem<WD_T_F16> {
+  typedef uint16_t type;
+  static constexpr int W = 8;
+  static __device__ __forceinline__ void unpack(const u32x4 &w, float *x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = w[i];      // a bit cast of the vector's element itself reads element 0
+      const f32x2 p = __builtin_convertvector(__builtin_bit_cast(f16x2, v), f32x2);
+      x[2 * i] = p[0];
+      x[2 * i + 1] = p[1];
+    }
+  }
+  static __device__ __forceinline__ u32x4 pack(const float *x) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x2 p = {x[2 * i], x[2 * i + 1]};
+      w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, f16x2));
+    }
+    return w;
+  }
+  static __device__ __forceinline__ float to_float(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
+  static __device__ __forceinline__ uint16_t from_float(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+};
+
+// A row of odd length or stride starts anywhere: `head` elements up to the first 16-byte boundary, `nb` whole words, the rest.  The
+// at most 2 (W - 1) elements outside the words are dealt one to a lane (`edge`), so nothing outside the row is ever touched.
+template <int DT> struct Row {
+  typedef typename Elem<DT>::type type;
+  static constexpr int W = Elem<DT>::W;
+  const type *p;
+  int V, head, nb, rest;
+  __device__ __forceinline__ Row(const void *base, int64_t ld, int64_t r, int vocab) {
+    p = (const type *)base + r * ld;
+    V = vocab;
+    const int mis = (int)(((uintptr_t)p & 15) / sizeof(type));
+    head = min((W - mis) & (W - 1), V);
+    nb = (V - head) / W;
+    rest = V - head - nb * W;
+  }
+  __device__ __forceinline__ u32x4 word(int j) const { return *(const u32x4 *)(p + head + j * W); }
+  // the element outside the words that lane i takes, -1: none
+  __device__ __forceinline__ int edge(int i) const { return i < head ? i : i < head + rest ? i + nb * W : -1; }
+};
+// a word of -inf
+template <int DT> __device__ __forceinline__ u32x4 no_word() {
+  constexpr uint32_t v = DT == WD_T_F32 ? 0xff800000u : DT == WD_T_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+  return {v, v, v, v};
+}
+// all loads before the first use, and what was unpacked for one pass over the words is not kept in registers for the next
+template <int N> __device__ __forceinline__ void hold(u32x4 (&w)[N]) {
+#pragma unroll
+  for (int u = 0; u < N; ++u) asm volatile("" : "+v"(w[u]));
+}
+template <int DT> __device__ __forceinline__ void store_word(typename Elem<DT>::type *g, bool aligned, const float *x) {
+  if (aligned) {
+    *(u32x4 *)g = Elem<DT>::pack(x);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < Elem<DT>::W; ++i) g[i] = Elem<DT>::from_float(x[i]);
+}
+
+__device__ __forceinline__ float exp_rel(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * kLog2e); }
+
+// (m, s) of two parts of a row.  m is at least the lowest finite number, so a part of nothing but -inf is (lowest, 0).
+__device__ __forceinline__ void join(float &m, float &s, float m2, float s2) {
+  const float M = fmaxf(m, m2);
+  s = s * exp_rel(m, M) + s2 * exp_rel(m2, M);
+  m = M;
+}
+
+__device__ __forceinline__ void wave_join(float &m, float &s) {
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) join(m, s, __shfl_xor(m, o), __shfl_xor(s, o));
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+template <typename T> __device__ __forceinline__ T wave_sum(T v) {
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) v += __shfl_xor(v, o);
+  return v;
+}
+// sum over the workgroup in a fixed order, the same value in every lane; `lds`: one T per wavefront, reusable after the call
+template <int TH, typename T> __device__ __forceinline__ T block_sum(T v, T *lds) {
+  v = wave_sum(v);
+  if (TH == kWave) return v;
+  __syncthreads();
+  if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
+  __syncthreads();
+  T t = lds[0];
+#pragma unroll
+  for (int w = 1; w < TH / kWave; ++w) t += lds[w];
+  return t;
+}
+template <int TH> __device__ __forceinline__ float block_max(float v, float *lds) {
+  v = wave_max(v);
+  if (TH == kWave) return v;
+  __syncthreads();
+  if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
+  __syncthreads();
+  float t = lds[0];
+#pragma unroll
+  for (int w = 1; w < TH / kWave; ++w) t = fmaxf(t, lds[w]);
+  return t;
+}
+
+// sequence n as a range of rows that exist
+__device__ __forceinline__ void seq_range(const wd_seq_rows_t &q, int64_t n, int64_t &a, int64_t &b) {
+  a = min((int64_t)max(q.seq_offs[n], 0), q.rows);
+  b = max(a, min((int64_t)q.seq_offs[n + 1], q.rows));
+}
+// rows in front of the first and behind the last sequence
+__device__ __forceinline__ int64_t first_row(const wd_seq_rows_t &q) { return min((int64_t)max(q.seq_offs[0], 0), q.rows); }
+__device__ __forceinline__ int64_t last_row(const wd_seq_rows_t &q) { return min((int64_t)max(q.seq_offs[q.nseq], 0), q.rows); }
+__device__ __forceinline__ bool outside(const wd_seq_rows_t &q, int64_t r) { return r < first_row(q) || r >= last_row(q); }
+template <int TH> __device__ __forceinline__ void zero_outside(const wd_seq_rows_t &q, float *v) {
+  for (int64_t r = threadIdx.x; r < first_row(q); r += TH) v[r] = 0.f;
+  for (int64_t r = last_row(q) + threadIdx.x; r < q.rows; r += TH) v[r] = 0.f;
+}
+// workgroup (part, row): parts of a row are neighbours in x, rows fill y and z (a grid dimension holds 2^32 lanes)
+__device__ __forceinline__ int64_t block_row() { return (int64_t)blockIdx.z * gridDim.y + blockIdx.y; }
+__device__ __forceinline__ bool is_action(const wd_seq_rows_t &q, int32_t t) { return t >= 0 && t < q.vocab; }
+
+// ---- (m, s) of every part of every row: workgroup (row, part)
+template <int DT>
+__global__ void __launch_bounds__(256) k_row_stats(wd_seq_rows_t q, int32_t nsplit, float2 *__restrict__ part) {
+  constexpr int TH = 256, U = 4, W = Elem<DT>::W;
+  __shared__ float lm[TH / kWave], ls[TH / kWave];
+  const int64_t r = block_row();
+  const int z = (int)blockIdx.x;
+  if (r >= q.rows || outside(q, r) || !is_action(q, q.targets[r])) return;
+  const Row<DT> row(q.logits, q.ld, r, (int)q.vocab);
+  const int per = (row.nb + nsplit - 1) / nsplit;
+  const int j1 = min(row.nb, (z + 1) * per);
+  float m = kLowest, s = 0.f;
+  if (z == 0) {
+    const int e = row.edge(threadIdx.x);
+    if (e >= 0) {
+      const float x = Elem<DT>::to_float(row.p[e]);
+      m = fmaxf(m, x);
+      s = exp_rel(x, m);
+    }
+  }
+  for (int j = z * per + threadIdx.x; j < j1; j += TH * U) {
+    u32x4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      w[u] = no_word<DT>();
+      if (j + u * TH < j1) w[u] = row.word(j + u * TH);
+    }
+    hold(w);
+    float x[U * W], M = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) Elem<DT>::unpack(w[u], x + u * W);
+#pragma unroll
+    for (int i = 0; i < U * W; ++i) M = fmaxf(M, x[i]);
+    s *= exp_rel(m, M);
+    m = M;
+#pragma unroll
+    for (int i = 0; i < U * W; ++i) s += exp_rel(x[i], m);
+  }
+  wave_join(m, s);
+  if ((threadIdx.x & (kWave - 1)) == 0) {
+    lm[threadIdx.x / kWave] = m;
+    ls[threadIdx.x / kWave] = s;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < TH / kWave; ++w) join(m, s, lm[w], ls[w]);
+    part[r * nsplit + z] = make_float2(m, s);
+  }
+}
+
+// the row's parts joined, and its target's log-probability
+template <int DT>
+__device__ __forceinline__ float row_logp(const wd_seq_rows_t &q, int64_t r, int32_t t, int32_t nsplit, const float2 *part, float2 &ms) {
+  ms = part[r * nsplit];
+  for (int z = 1; z < nsplit; ++z) {
+    const float2 o = part[r * nsplit + z];
+    join(ms.x, ms.y, o.x, o.y);
+  }
+  const float x = Elem<DT>::to_float(((const typename Elem<DT>::type *)q.logits)[r * q.ld + t]);
+  return (x - ms.x) - logf(ms.y);
+}
+
+// sum and number of the actions of rows [a, b); token_logp and the joined (m, s) of each row stored on the way
+template <int DT, int TH>
+__device__ __forceinline__ void seq_logp(const wd_seq_rows_t &q, int64_t a, int64_t b, int32_t nsplit, const float2 *part, float *token,
+                                         float2 *stat, double &sum, int32_t &count, double *ld, int32_t *li) {
+  double v = 0.0;      // long sums in 64 bits: a sequence of a thousand items sums to thousands, its pair's difference to units
+  int32_t c = 0;
+  for (int64_t r = a + threadIdx.x; r < b; r += TH) {
+    const int32_t t = q.targets[r];
+    float lp = 0.f;
+    if (is_action(q, t)) {
+      float2 ms;
+      lp = row_logp<DT>(q, r, t, nsplit, part, ms);
+      if (stat) stat[r] = ms;
+      v += lp;
+      ++c;
+    }
+    if (token) token[r] = lp;
+  }
+  sum = block_sum<TH>(v, ld);
+  count = block_sum<TH>(c, li);
+}
+
+// ---- scores: workgroup n = sequence n; one more zeroes token_logp behind the last sequence
+template <int DT>
+__global__ void __launch_bounds__(256)
+k_seq_logp(wd_seq_rows_t q, int32_t nsplit, int32_t length_norm, const float2 *__restrict__ part, float *__restrict__ token,
+           float *__restrict__ seq) {
+  constexpr int TH = 256;
+  __shared__ double ld[TH / kWave];
+  __shared__ int32_t li[TH / kWave];
+  const int64_t n = block_row();
+  if (n == q.nseq) zero_outside<TH>(q, token);
+  if (n >= q.nseq) return;
+  int64_t a, b;
+  seq_range(q, n, a, b);
+  double sum;
+  int32_t count;
+  seq_logp<DT, TH>(q, a, b, nsplit, part, token, nullptr, sum, count, ld, li);
+  if (threadIdx.x == 0) seq[n] = (float)(length_norm ? sum / max(count, 1) : sum);
+}
+
+// log sigma(h) without overflow on either side
+__device__ __forceinline__ double log_sigmoid(double h) { return fmin(h, 0.0) - log1p(exp(-fabs(h))); }
+
+// ---- pairs: workgroup i = sequences 2i (chosen) and 2i + 1 (rejected); leaves dloss/dlp of every row.  The scalars of a pair are
+// computed in 64 bits: there are a few of them, and the coefficient multiplies whole rows.
+template <int DT>
+__global__ void __launch_bounds__(256)
+k_pref_pairs(wd_seq_rows_t q, wd_pref_t o, int32_t nsplit, const float2 *__restrict__ part, float2 *__restrict__ stat,
+             float *__restrict__ coef) {
+  constexpr int TH = 256;
+  __shared__ double ld[TH / kWave];
+  __shared__ int32_t li[TH / kWave];
+  const int64_t i = block_row();
+  if (i == q.nseq / 2) zero_outside<TH>(q, o.token_logp);
+  if (i >= q.nseq / 2) return;
+  int64_t a[2], b[2];
+  double lp[2];
+  int32_t n[2];
+  for (int k = 0; k < 2; ++k) {
+    seq_range(q, 2 * i + k, a[k], b[k]);
+    seq_logp<DT, TH>(q, a[k], b[k], nsplit, part, o.token_logp, stat, lp[k], n[k], ld, li);
+    n[k] = o.length_norm ? max(n[k], 1) : 1;
+    lp[k] /= n[k];
+  }
+  double d = lp[0] - lp[1];
+  if (o.ref_logp) d -= (double)o.ref_logp[2 * i] - (double)o.ref_logp[2 * i + 1];
+  const double w = (double)o.scale * (o.weights ? (double)o.weights[i] : 1.0);
+  double loss, slope;
+  if (o.kind == WD_PREF_LOGISTIC) {
+    const double h = (double)o.beta * d - (double)o.margin, eps = (double)o.label_smoothing;
+    loss = -(1.0 - eps) * log_sigmoid(h) - eps * log_sigmoid(-h);
+    // dloss/dh = sigma(h) - (1 - eps), as eps sigma(h) - (1 - eps) sigma(-h): no cancellation where the pair is settled
+    const double e = exp(-fabs(h)), big = 1.0 / (1.0 + e), small = e / (1.0 + e);
+    slope = (double)o.beta * (eps * (h >= 0 ? big : small) - (1.0 - eps) * (h >= 0 ? small : big));
+  } else {
+    const double h = d - 0.5 / (double)o.beta;
+    loss = h * h;
+    slope = 2.0 * h;
+  }
+  if (threadIdx.x == 0) {
+    o.pair_loss[i] = (float)loss;
+    o.difference[i] = (float)d;
+    o.seq_logp[2 * i] = (float)lp[0];
+    o.seq_logp[2 * i + 1] = (float)lp[1];
+  }
+  for (int k = 0; k < 2; ++k) {
+    const float c = (float)((k ? -slope : slope) * w * (double)o.grad_scale / n[k]);
+    for (int64_t r = a[k] + threadIdx.x; r < b[k]; r += TH) coef[r] = c;
+  }
+}
+
+// ---- gradient of the logits from (m, s, coefficient) of each row: workgroup (row, part); the last one adds the loss up
+template <int TH> __device__ __forceinline__ void weighted_sum(const float *v, const float *w, int64_t n, double scale, float *out, double *ld) {
+  double t = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += TH) t += (double)v[i] * (w ? (double)w[i] : 1.0);
+  t = block_sum<TH>(t, ld);
+  if (threadIdx.x == 0) *out = (float)(t * scale);
+}
+
+// part z of a row's gradient; c = 0 for a row that is no action (m = 0, s = 1; its logits are not read)
+template <int DT, int TH>
+__device__ __forceinline__ void grad_part(const Row<DT> &row, typename Elem<DT>::type *g, int z, int nsplit, bool action, int32_t t, float m,
+                                          float s, float c) {
+  constexpr int W = Elem<DT>::W, U = 4;
+  const int per = (row.nb + nsplit - 1) / nsplit;
+  const int j1 = min(row.nb, (z + 1) * per), jt = t < row.head ? -1 : (t - row.head) / W;
+  typename Elem<DT>::type *gb = g + row.head;
+  const bool aligned = ((uintptr_t)gb & 15) == 0;
+  const float k = -c / s;
+  if (z == 0) {
+    const int e = row.edge(threadIdx.x);
+    if (e >= 0) g[e] = Elem<DT>::from_float(action ? k * exp_rel(Elem<DT>::to_float(row.p[e]), m) + (e == t ? c : 0.f) : 0.f);
+  }
+  float x[W];
+  for (int j = z * per + threadIdx.x; j < j1; j += TH * U) {
+    u32x4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+    {
+      w[u] = no_word<DT>();
+      if (action && j + u * TH < j1) w[u] = row.word(j + u * TH);
+    }
+    hold(w);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int ju = j + u * TH;
+      if (ju >= j1) break;
+      if (action) {
+        Elem<DT>::unpack(w[u], x);
+#pragma unroll
+        for (int i = 0; i < W; ++i) x[i] = k * exp_rel(x[i], m);
+        if (ju == jt) {
+#pragma unroll
+          for (int i = 0; i < W; ++i) x[i] += row.head + ju * W + i == t ? c : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) x[i] = 0.f;
+      }
+      store_word<DT>(gb + ju * W, aligned, x);
+    }
+  }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256)
+k_logits_grad(wd_seq_rows_t q, void *dlogits, int64_t ldg, int32_t zero_tail, int32_t nsplit, const float2 *__restrict__ stat,
+              const float *__restrict__ coef, const float *__restrict__ pair_loss, const float *__restrict__ weights, double scale,
+              float *__restrict__ loss) {
+  constexpr int TH = 256;
+  __shared__ double ld[TH / kWave];
+  const int64_t r = block_row();
+  const int z = (int)blockIdx.x;
+  if (r == q.rows && z == 0 && loss) weighted_sum<TH>(pair_loss, weights, q.nseq / 2, scale, loss, ld);
+  if (r >= q.rows) return;
+  const bool tail = outside(q, r);
+  if (tail && !zero_tail) return;
+  const int32_t t = q.targets[r];
+  const bool action = !tail && is_action(q, t);
+  const Row<DT> row(q.logits, q.ld, r, (int)q.vocab);
+  const float2 ms = action ? stat[r] : make_float2(0.f, 1.f);
+  grad_part<DT, TH>(row, (typename Elem<DT>::type *)dlogits + r * ldg, z, nsplit, action, t, ms.x, ms.y, action ? coef[r] : 0.f);
+}
+
+// ---- clipped policy loss
+// weights of the rows (sum | mean over actions | mean over sequences of means) and the advantages by row
+template <int TH>
+__global__ void __launch_bounds__(TH) k_policy_rows(wd_seq_rows_t q, wd_policy_t o, float *__restrict__ w, float *__restrict__ adv) {
+  __shared__ int32_t li[TH / kWave];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  int32_t actions = 0, seqs = 0;
+  // a wavefront per sequence counts its actions; one workgroup, so the totals need no second launch
+  for (int64_t n = wave; n < q.nseq; n += TH / kWave) {
+    int64_t a, b;
+    seq_range(q, n, a, b);
+    int32_t c = 0;
+    for (int64_t r = a + lane; r < b; r += kWave) c += is_action(q, q.targets[r]);
+    c = wave_sum(c);
+    const float inv = o.reduction == WD_POLICY_SEQUENCE_MEAN ? 1.0f / (float)max(c, 1) : 1.0f;
+    const float av = o.adv_per_row ? 0.f : o.advantages[n];
+    for (int64_t r = a + lane; r < b; r += kWave) {
+      w[r] = inv;
+      adv[r] = o.adv_per_row ? o.advantages[r] : av;
+    }
+    if (lane == 0) {
+      actions += c;
+      seqs += c > 0;
+    }
+  }
+  actions = block_sum<TH>(actions, li);
+  seqs = block_sum<TH>(seqs, li);
+  if (threadIdx.x == 0) {
+    const int32_t d = o.reduction == WD_POLICY_TOKEN_MEAN ? actions : o.reduction == WD_POLICY_SEQUENCE_MEAN ? seqs : 1;
+    w[q.rows] = 1.0f / (float)max(d, 1);
+  }
+}
+
+struct PolicyRow {
+  float loss, kl, clipped, slope;
+};
+// rho = e^(lp - old); the surrogate takes the smaller of rho A and clip(rho) A and has no slope where that is the clipped one;
+// k = e^(ref - lp) - (ref - lp) - 1 >= 0 estimates KL(policy || reference) from the sampled item (expm1: small differences keep bits)
+__device__ __forceinline__ PolicyRow policy_row(const wd_policy_t &o, float lp, float old, float adv, float ref) {
+  PolicyRow p;
+  const float rho = expf(lp - old);
+  const float a = rho * adv, b = fminf(fmaxf(rho, 1.0f - o.clip_low), 1.0f + o.clip_high) * adv;
+  const bool out = a > b;
+  p.loss = -(out ? b : a);
+  p.slope = out ? 0.f : -a;
+  p.clipped = out ? 1.f : 0.f;
+  p.kl = 0.f;
+  if (o.ref_logp) {
+    const float d = ref - lp, e = expm1f(d);
+    p.kl = e - d;
+    p.loss += o.kl_coef * p.kl;
+    p.slope -= o.kl_coef * e;
+  }
+  return p;
+}
+
+// the whole row in registers between its statistics and its gradient: one read and one write of the logits, workgroup = row
+template <int DT, int TH, int NV>
+__global__ void __launch_bounds__(TH)
+k_policy_resident(wd_seq_rows_t q, wd_policy_t o, const float *__restrict__ w, const float *__restrict__ adv, float *__restrict__ rows3) {
+  constexpr int W = Elem<DT>::W;
+  typedef typename Elem<DT>::type type;
+  __shared__ float lf[TH / kWave], lg[TH / kWave];
+  const int64_t r = block_row();
+  if (r >= q.rows) return;
+  const bool tail = outside(q, r);
+  if (tail && threadIdx.x == 0) {
+    o.token_logp[r] = 0.f;
+    rows3[r] = rows3[q.rows + r] = rows3[2 * q.rows + r] = 0.f;
+  }
+  if (tail && !o.zero_tail) return;
+  const int32_t t = q.targets[r];
+  const Row<DT> row(q.logits, q.ld, r, (int)q.vocab);
+  type *g = (type *)o.dlogits + r * o.ld_dlogits;
+  if (tail || !is_action(q, t)) {
+    if (threadIdx.x == 0 && !tail) {
+      o.token_logp[r] = 0.f;
+      rows3[r] = rows3[q.rows + r] = rows3[2 * q.rows + r] = 0.f;
+    }
+    if (o.dlogits) grad_part<DT, TH>(row, g, 0, 1, false, -1, 0.f, 1.f, 0.f);
+    return;
+  }
+  u32x4 v[NV];
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    v[u] = no_word<DT>();
+    if ((int)threadIdx.x + u * TH < row.nb) v[u] = row.word(threadIdx.x + u * TH);
+  }
+  const int e = row.edge(threadIdx.x);
+  const float xe = e >= 0 ? Elem<DT>::to_float(row.p[e]) : -INFINITY;
+  const float xt = Elem<DT>::to_float(row.p[t]);
+  const float wr = w[r] * w[q.rows], ar = adv[r], old = o.old_logp[r], ref = o.ref_logp ? o.ref_logp[r] : 0.f;
+  hold(v);
+  float x[W], m = fmaxf(kLowest, xe);
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    Elem<DT>::unpack(v[u], x);
+#pragma unroll
+    for (int i = 0; i < W; ++i) m = fmaxf(m, x[i]);
+  }
+  m = block_max<TH>(m, lf);
+  hold(v);
+  float s = exp_rel(xe, m);
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    Elem<DT>::unpack(v[u], x);
+#pragma unroll
+    for (int i = 0; i < W; ++i) s += exp_rel(x[i], m);
+  }
+  s = block_sum<TH>(s, lg);
+  const float lp = (xt - m) - logf(s);
+  const PolicyRow p = policy_row(o, lp, old, ar, ref);
+  if (threadIdx.x == 0) {
+    o.token_logp[r] = lp;
+    rows3[r] = p.loss * wr;
+    rows3[q.rows + r] = p.kl * wr;
+    rows3[2 * q.rows + r] = p.clipped * wr;
+  }
+  if (!o.dlogits) return;
+  const float c = p.slope * wr * o.grad_scale, k = -c / s;
+  const int jt = t < row.head ? -1 : (t - row.head) / W;
+  type *gb = g + row.head;
+  const bool aligned = ((uintptr_t)gb & 15) == 0;
+  if (e >= 0) g[e] = Elem<DT>::from_float(k * exp_rel(xe, m) + (e == t ? c : 0.f));
+  hold(v);
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int j = threadIdx.x + u * TH;
+    if (j >= row.nb) break;
+    Elem<DT>::unpack(v[u], x);
+#pragma unroll
+    for (int i = 0; i < W; ++i) x[i] = k * exp_rel(x[i], m);
+    if (j == jt) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) x[i] += row.head + j * W + i == t ? c : 0.f;
+    }
+    store_word<DT>(gb + j * W, aligned, x);
+  }
+}
+
+// rows whose statistics came in parts: loss and coefficient of each row, a lane per row
+template <int DT>
+__global__ void __launch_bounds__(256)
+k_policy_join(wd_seq_rows_t q, wd_policy_t o, int32_t nsplit, const float2 *__restrict__ part, const float *__restrict__ w,
+              const float *__restrict__ adv, float2 *__restrict__ stat, float *__restrict__ coef, float *__restrict__ rows3) {
+  const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (r >= q.rows) return;
+  float lp = 0.f, wr = 0.f, c = 0.f;
+  PolicyRow p = {0.f, 0.f, 0.f, 0.f};
+  const int32_t t = q.targets[r];
+  if (!outside(q, r) && is_action(q, t)) {
+    float2 ms;
+    lp = row_logp<DT>(q, r, t, nsplit, part, ms);
+    stat[r] = ms;
+    wr = w[r] * w[q.rows];
+    p = policy_row(o, lp, o.old_logp[r], adv[r], o.ref_logp ? o.ref_logp[r] : 0.f);
+    c = p.slope * wr * o.grad_scale;
+  }
+  coef[r] = c;
+  o.token_logp[r] = lp;
+  rows3[r] = p.loss * wr;
+  rows3[q.rows + r] = p.kl * wr;
+  rows3[2 * q.rows + r] = p.clipped * wr;
+}
+
+// out[k] = sum of rows3[k][0..rows), in a fixed order
+__global__ void __launch_bounds__(1024) k_policy_sums(const float *__restrict__ rows3, int64_t rows, float *__restrict__ out) {
+  __shared__ double ld[1024 / kWave];
+  weighted_sum<1024>(rows3 + blockIdx.x * rows, nullptr, rows, 1.0, out + blockIdx.x, ld);
+}
+
+// ---- host side
+int check_rows(const char *who, const wd_seq_rows_t *q) {
+  if (!q) { set_error("%s: null argument", who); return WD_ERR_INVALID; }
+  if (q->rows < 0 || q->nseq < 0 || q->vocab < 1) { set_error("%s: bad sizes (rows %lld, sequences %lld, vocab %lld)", who, (long long)q->rows, (long long)q->nseq, (long long)q->vocab); return WD_ERR_INVALID; }
+  if (q->dtype != WD_T_F32 && q->dtype != WD_T_F16 && q->dtype != WD_T_BF16) { set_error("%s: bad element type %d", who, q->dtype); return WD_ERR_INVALID; }
+  if (q->vocab > INT32_MAX / 2 || q->rows > INT32_MAX / 2 || q->nseq > INT32_MAX / 4) { set_error("%s: more than 2^30 rows or items or 2^29 sequences", who); return WD_ERR_UNSUPPORTED; }
+  if (q->ld < q->vocab) { set_error("%s: row stride %lld below the row length %lld", who, (long long)q->ld, (long long)q->vocab); return WD_ERR_INVALID; }
+  if (!q->seq_offs || (q->rows > 0 && (!q->logits || !q->targets))) { set_error("%s: null pointer", who); return WD_ERR_INVALID; }
+  const int size = q->dtype == WD_T_F32 ? 4 : 2;
+  if ((uintptr_t)q->logits % size) { set_error("%s: logits not aligned to their element size", who); return WD_ERR_INVALID; }
+  return WD_OK;
+}
+
+int words(const wd_seq_rows_t &q) { return (int)(q.vocab / (q.dtype == WD_T_F32 ? 4 : 8)); }      // whole words of a row, at most
+
+// parts of a row: enough workgroups for every CU where there are few rows, at least 4 KB each
+int row_split(const wd_seq_rows_t &q) {
+  if (q.rows < 1) return 1;
+  const int64_t want = ceil_div(1024, q.rows), most = words(q) / 256;
+  return (int)(want < 1 || most < 1 ? 1 : want < most ? want : most);
+}
+// parts of a row for the gradient pass, 16 KB each: a lane has four words in flight
+int grad_split(const wd_seq_rows_t &q) { return words(q) <= 1024 ? 1 : (int)ceil_div(words(q), 1024); }
+
+dim3 row_grid(int64_t rows, int parts) {
+  const int64_t y = rows < 32768 ? rows : 32768;
+  return dim3((unsigned)parts, (unsigned)y, (unsigned)ceil_div(rows, y));
+}
+
+struct Work {      // [rows * nsplit] (m, s) parts | [rows] (m, s) | [rows] coefficients | 3 [rows] | [rows + 1] weights | [rows] advantages
+  float2 *part, *stat;
+  float *coef, *rows3, *w, *adv;
+  Work(const wd_seq_rows_t &q, float *p) {
+    const int64_t T = q.rows;
+    part = (float2 *)p;
+    stat = part + T * row_split(q);
+    coef = (float *)(stat + T);
+    rows3 = coef + T;
+    w = rows3 + 3 * T;
+    adv = w + T + 1;
+  }
+};
+
+template <typename F> void by_type(int32_t dtype, F f) {
+  if (dtype == WD_T_F32) f(std::integral_constant<int, WD_T_F32>());
+  else if (dtype == WD_T_F16) f(std::integral_constant<int, WD_T_F16>());
+  else f(std::integral_constant<int, WD_T_BF16>());
+}
+
+void launch_stats(const wd_seq_rows_t &q, int nsplit, float2 *part, hipStream_t st) {
+  if (q.rows < 1) return;
+  by_type(q.dtype, [&](auto dt) { k_row_stats<decltype(dt)::value><<<row_grid(q.rows, nsplit), 256, 0, st>>>(q, nsplit, part); });
+}
+
+}  // namespace
+
+extern "C" int64_t wd_policy_workspace_floats(const wd_seq_rows_t *rows) {
+  const int rc = check_rows(__func__, rows);
+  if (rc) return rc;
+  return rows->rows * (2 * (int64_t)row_split(*rows) + 2 + 1 + 3 + 1 + 1) + 1;
+}
+
+extern "C" int wd_seq_logp(const wd_seq_rows_t *rows, int32_t length_norm, float *token_logp, float *seq_logp, float *ws,
+                           wd_stream_t stream) {
+  if (const int rc = check_rows(__func__, rows)) return rc;
+  const wd_seq_rows_t q = *rows;
+  WD_REQUIRE((token_logp || !q.rows) && (seq_logp || !q.nseq) && ws, "null pointer");
+  hipStream_t st = as_stream(stream);
+  const Work k(q, ws);
+  const int ns = row_split(q);
+  launch_stats(q, ns, k.part, st);
+  by_type(q.dtype, [&](auto dt) {
+    k_seq_logp<decltype(dt)::value><<<row_grid(q.nseq + 1, 1), 256, 0, st>>>(q, ns, length_norm, k.part, token_logp, seq_logp);
+  });
+  return check_launch(__func__);
+}
+
+extern "C" int wd_pref_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_pref_t *opts, float *ws, wd_stream_t stream) {
+  if (const int rc = check_rows(__func__, rows)) return rc;
+  WD_REQUIRE(opts && ws, "null argument");
+  const wd_seq_rows_t q = *rows;
+  const wd_pref_t o = *opts;
+  WD_REQUIRE(q.nseq % 2 == 0, "an odd number of sequences: pair i is sequences 2i (chosen) and 2i + 1 (rejected)");
+  WD_REQUIRE(o.kind == WD_PREF_LOGISTIC || o.kind == WD_PREF_SQUARE, "bad loss kind");
+  WD_REQUIRE(o.beta > 0.f, "beta must be positive");
+  WD_REQUIRE(o.label_smoothing >= 0.f && o.label_smoothing < 0.5f, "label_smoothing must be in [0, 0.5)");
+  WD_REQUIRE(o.kind == WD_PREF_LOGISTIC || (o.label_smoothing == 0.f && o.margin == 0.f), "label_smoothing and margin belong to the logistic loss");
+  WD_REQUIRE(o.loss && (q.nseq == 0 || (o.pair_loss && o.difference && o.seq_logp)) && (q.rows == 0 || o.token_logp), "null output");
+  WD_REQUIRE(!o.dlogits || o.ld_dlogits >= q.vocab, "row stride of the gradient below the row length");
+  WD_REQUIRE((uintptr_t)o.dlogits % (q.dtype == WD_T_F32 ? 4 : 2) == 0, "gradient not aligned to its element size");
+  hipStream_t st = as_stream(stream);
+  const Work k(q, ws);
+  const int ns = row_split(q), gs = grad_split(q);
+  launch_stats(q, ns, k.part, st);
+  wd_seq_rows_t last = q;
+  if (!o.dlogits) last.rows = 0;      // the loss alone
+  by_type(q.dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    k_pref_pairs<DT><<<row_grid(q.nseq / 2 + 1, 1), 256, 0, st>>>(q, o, ns, k.part, k.stat, k.coef);
+    k_logits_grad<DT><<<row_grid(last.rows + 1, gs), 256, 0, st>>>(last, o.dlogits, o.ld_dlogits, o.zero_tail, gs, k.stat, k.coef,
+                                                                            o.pair_loss, o.weights, (double)o.scale, o.loss);
+  });
+  return check_launch(__func__);
+}
+
+extern "C" int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy_t *opts, float *ws, wd_stream_t stream) {
+  if (const int rc = check_rows(__func__, rows)) return rc;
+  WD_REQUIRE(opts && ws, "null argument");
+  const wd_seq_rows_t q = *rows;
+  const wd_policy_t o = *opts;
+  WD_REQUIRE(o.reduction == WD_POLICY_SUM || o.reduction == WD_POLICY_TOKEN_MEAN || o.reduction == WD_POLICY_SEQUENCE_MEAN, "bad reduction");
+  WD_REQUIRE(o.clip_low >= 0.f && o.clip_low <= 1.f && o.clip_high >= 0.f, "clip range: low in [0, 1], high >= 0");
+  WD_REQUIRE(o.kl_coef == 0.f || o.ref_logp || q.rows == 0, "a KL term needs the reference policy's log-probabilities");
+  WD_REQUIRE(o.sums && (q.rows == 0 || (o.old_logp && o.token_logp)) && (o.advantages || (o.adv_per_row ? q.rows : q.nseq) == 0), "null pointer");
+  WD_REQUIRE(!o.dlogits || o.ld_dlogits >= q.vocab, "row stride of the gradient below the row length");
+  WD_REQUIRE((uintptr_t)o.dlogits % (q.dtype == WD_T_F32 ? 4 : 2) == 0, "gradient not aligned to its element size");
+  hipStream_t st = as_stream(stream);
+  const Work k(q, ws);
+  k_policy_rows<1024><<<1, 1024, 0, st>>>(q, o, k.w, k.adv);
+  const int nw = words(q);
+  if (q.rows > 0) {
+    by_type(q.dtype, [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      const dim3 grid = row_grid(q.rows, 1);
+      if (nw <= 256) k_policy_resident<DT, 256, 1><<<grid, 256, 0, st>>>(q, o, k.w, k.adv, k.rows3);
+      else if (nw <= 1024) k_policy_resident<DT, 256, 4><<<grid, 256, 0, st>>>(q, o, k.w, k.adv, k.rows3);
+      else if (nw <= 4096) k_policy_resident<DT, 512, 8><<<grid, 512, 0, st>>>(q, o, k.w, k.adv, k.rows3);
+      else if (nw <= 16384) k_policy_resident<DT, 1024, 16><<<grid, 1024, 0, st>>>(q, o, k.w, k.adv, k.rows3);
+      else {
+        const int ns = row_split(q), gs = grad_split(q);
+        launch_stats(q, ns, k.part, st);
+        k_policy_join<DT><<<dim3((unsigned)ceil_div(q.rows, 256)), 256, 0, st>>>(q, o, ns, k.part, k.w, k.adv, k.stat, k.coef, k.rows3);
+        if (o.dlogits)
+          k_logits_grad<DT><<<row_grid(q.rows, gs), 256, 0, st>>>(q, o.dlogits, o.ld_dlogits, o.zero_tail, gs, k.stat, k.coef, nullptr,
+                                                                           nullptr, 0.0, nullptr);
+      }
+    });
+  }
+  k_policy_sums<<<3, 1024, 0, st>>>(k.rows3, q.rows, o.sums);
+  return check_launch(__func__);
+}

@@ -1,0 +1,153 @@
+"""Heads of a policy over items: scores of chosen items, a preference loss over pairs of sequences, a clipped policy loss.
+
+The reference knows one head, the sigmoid cross entropy of a click (wd_bce_sum_fwd_bwd); these stand beside it for models whose logits
+are a row of scores per position.  Each call is one entry of the C ABI (include/wd_hip.h, csrc/policy_loss.hip): loss AND gradient of
+the logits, launched on the current stream of the logits' device, nothing read back, so every call can be captured into a hipGraph.
+There is no autograd in between: `dlogits` goes to the backward pass of whatever made the logits (wd_gemm_*, the engine's towers).
+
+Layout of a batch: `logits` [rows, vocab] (fp32, fp16 or bf16; rows may be strided, items contiguous), `targets` int32 [rows] (outside
+[0, vocab), e.g. -1: the position is no action of the policy), `seq_offs` int32 [sequences + 1], a CSR over the rows.  Results and
+workspace come from torch's caching allocator on the current stream: calls on several streams share nothing.  Every tensor has to be
+ready on the current stream; one that another stream uses later is the caller's to record there.
+"""
+import struct
+from collections import namedtuple
+
+import torch
+
+from . import capi
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # WD_T_*
+_ROWS = struct.Struct("=QqqqQQqii")                                   # wd_seq_rows_t
+_PREF = struct.Struct("=QQQQQQQQqfffffiii")                           # wd_pref_t
+_POLICY = struct.Struct("=QQQQQQqffffiiii")                           # wd_policy_t
+
+PREFERENCE_KINDS = {"logistic": 0, "square": 1}                       # WD_PREF_*
+POLICY_REDUCTIONS = {"sum": 0, "token_mean": 1, "sequence_mean": 2}   # WD_POLICY_*
+
+SequenceLogp = namedtuple("SequenceLogp", "token_logp seq_logp")
+PreferenceLoss = namedtuple("PreferenceLoss", "loss pair_loss difference seq_logp token_logp dlogits")
+PolicyLoss = namedtuple("PolicyLoss", "loss kl clipped token_logp dlogits")
+
+
+def _vector(name, t, n, dtype, device):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device != device or (n > 1 and t.stride(0) != 1):
+        raise ValueError("%s: a contiguous %s tensor of %d values on %s is wanted, got %s" % (name, dtype, n, device, _what(t)))
+    return t.data_ptr()
+
+
+def _what(t):
+    return "%s %s on %s" % (t.dtype, list(t.shape), t.device) if isinstance(t, torch.Tensor) else repr(t)
+
+
+def _rows(logits, targets, seq_offs):
+    """wd_seq_rows_t of a batch, packed, after the checks that need no device."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _DTYPES:
+        raise ValueError("logits: a [rows, vocab] tensor of fp32, fp16 or bf16 is wanted, got %s" % _what(logits))
+    T, V = logits.shape
+    if V < 1 or (T and V > 1 and logits.stride(1) != 1) or (T > 1 and logits.stride(0) < V):
+        raise ValueError("logits: at least one item, items contiguous, rows not overlapping are wanted, got %s with strides %s" % (_what(logits), logits.stride()))
+    if not logits.is_cuda:
+        raise capi.WdError("policy heads need a GPU (MI355X / gfx950); there is no CPU fallback: logits are on %s" % logits.device)
+    dev = logits.device
+    pt = _vector("targets", targets, T, torch.int32, dev)
+    if not isinstance(seq_offs, torch.Tensor) or seq_offs.dim() != 1 or seq_offs.shape[0] < 1:
+        raise ValueError("seq_offs: an int32 tensor of sequences + 1 offsets is wanted, got %s" % _what(seq_offs))
+    N = seq_offs.shape[0] - 1
+    po = _vector("seq_offs", seq_offs, N + 1, torch.int32, dev)
+    ld = logits.stride(0) if T > 1 else V
+    return _ROWS.pack(logits.data_ptr(), ld, T, V, pt, po, N, _DTYPES[logits.dtype], 0), T, V, N, dev
+
+
+def _gradient(dlogits, logits):
+    """(tensor or None, pointer, row stride, zero_tail) of the gradient: True: a new tensor, None / False: the loss alone."""
+    if dlogits is True:
+        g = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return g, g.data_ptr(), logits.shape[1], 1       # rows of no sequence: zeros
+    if dlogits is None or dlogits is False:
+        return None, 0, 0, 0
+    if not isinstance(dlogits, torch.Tensor) or dlogits.shape != logits.shape or dlogits.dtype != logits.dtype or dlogits.device != logits.device:
+        raise ValueError("dlogits: a tensor like logits (%s) is wanted, got %s" % (_what(logits), _what(dlogits)))
+    T, V = dlogits.shape
+    if (T and V > 1 and dlogits.stride(1) != 1) or (T > 1 and dlogits.stride(0) < V):
+        raise ValueError("dlogits: items contiguous, rows not overlapping are wanted, got strides %s" % (dlogits.stride(),))
+    return dlogits, dlogits.data_ptr(), dlogits.stride(0) if T > 1 else V, 0
+
+
+def _call(name, dev, T, rows, *args):
+    """One entry of the C ABI on the current stream of `dev`, its workspace the last argument but the stream."""
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _call(name, dev, T, rows, *args)
+    n = capi.call("wd_policy_workspace_floats", rows)
+    if n < 0:
+        raise capi.WdError("wd_policy_workspace_floats failed (%d): %s" % (n, capi.load().wd_last_error().decode()))
+    ws = torch.empty(n, dtype=torch.float32, device=dev)
+    capi.call(name, rows, *args, ws.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+
+
+def sequence_logp(logits, targets, seq_offs, length_norm=False):
+    """Log-probabilities of the chosen items: token_logp[r] = log softmax(logits[r])[targets[r]] (0 where the position is no action) and
+    seq_logp[n], their sum over sequence n (length_norm: their mean over its actions; 0 without any)."""
+    rows, T, V, N, dev = _rows(logits, targets, seq_offs)
+    out = torch.empty(T + N, dtype=torch.float32, device=dev)
+    p = out.data_ptr()
+    _call("wd_seq_logp", dev, T, rows, int(bool(length_norm)), p, p + 4 * T)
+    return SequenceLogp(out[:T], out[T:])
+
+
+def preference_loss(logits, targets, seq_offs, ref_logp=None, weights=None, beta=0.1, kind="logistic", margin=0.0, label_smoothing=0.0,
+                    length_norm=False, reduction="sum", grad_scale=1.0, dlogits=True):
+    """Preference loss of pairs of sequences, 2i chosen and 2i + 1 rejected, with the gradient of the logits.
+
+    d = (LP[2i] - ref_logp[2i]) - (LP[2i + 1] - ref_logp[2i + 1]) with LP as seq_logp of sequence_logp (which also makes ref_logp, from
+    the reference model's logits); kind "logistic": -(1 - label_smoothing) log sigma(h) - label_smoothing log sigma(-h), h = beta d -
+    margin; "square": (d - 1 / (2 beta))^2.  loss = sum or mean over the pairs of weights[i] times that.
+    dlogits: True (a new tensor), a tensor like logits (rows of no sequence are left as they were; it may be `logits` itself), or None
+    (the loss alone); it holds grad_scale times the gradient."""
+    rows, T, V, N, dev = _rows(logits, targets, seq_offs)
+    if kind not in PREFERENCE_KINDS or reduction not in ("sum", "mean"):
+        raise ValueError("kind is one of %s, reduction sum or mean: got %r, %r" % (sorted(PREFERENCE_KINDS), kind, reduction))
+    if N % 2:
+        raise ValueError("preference_loss: %d sequences: pair i is sequences 2i (chosen) and 2i + 1 (rejected)" % N)
+    pr = _vector("ref_logp", ref_logp, N, torch.float32, dev) if ref_logp is not None else 0
+    pw = _vector("weights", weights, N // 2, torch.float32, dev) if weights is not None else 0
+    g, pg, ldg, tail = _gradient(dlogits, logits)
+    P = N // 2
+    out = torch.empty(1 + 2 * P + N + T, dtype=torch.float32, device=dev)
+    p = out.data_ptr()
+    opts = _PREF.pack(pr, pw, p, p + 4, p + 4 * (1 + P), p + 4 * (1 + 2 * P), p + 4 * (1 + 2 * P + N), pg, ldg, beta, margin, label_smoothing,
+                      1.0 / max(P, 1) if reduction == "mean" else 1.0, grad_scale, PREFERENCE_KINDS[kind], int(bool(length_norm)), tail)
+    _call("wd_pref_loss_fwd_bwd", dev, T, rows, opts)
+    loss, pair, diff, seq, tok = out.split((1, P, P, N, T))
+    return PreferenceLoss(loss.view(()), pair, diff, seq, tok, g)
+
+
+def policy_loss(logits, targets, seq_offs, old_logp, advantages, ref_logp=None, per_row=None, clip=(0.2, 0.2), kl_coef=0.0, reduction="token_mean",
+                grad_scale=1.0, dlogits=True):
+    """Clipped policy loss with a KL term to a reference policy, with the gradient of the logits.
+
+    rho = exp(token_logp - old_logp), A = advantages by row or by sequence; each action gives -min(rho A, clip(rho, 1 - clip[0], 1 +
+    clip[1]) A) + kl_coef k with k = exp(ref_logp - token_logp) - (ref_logp - token_logp) - 1.  reduction: "sum", "token_mean" (over all
+    actions) or "sequence_mean" (mean over the sequences that have an action of their means).  Returns the loss, and reduced the same way
+    k and the share of actions whose clipped side was taken.  old_logp and ref_logp are token_logp of sequence_logp, [rows].
+    dlogits as in preference_loss.  per_row: whether advantages are [rows] or [sequences]; None: told by their number, which has to tell."""
+    rows, T, V, N, dev = _rows(logits, targets, seq_offs)
+    if reduction not in POLICY_REDUCTIONS:
+        raise ValueError("reduction is one of %s: got %r" % (sorted(POLICY_REDUCTIONS), reduction))
+    po = _vector("old_logp", old_logp, T, torch.float32, dev)
+    if per_row is None:
+        if T == N:
+            raise ValueError("policy_loss: %d rows and as many sequences: say with per_row which of them the advantages belong to" % T)
+        per_row = isinstance(advantages, torch.Tensor) and advantages.dim() == 1 and advantages.shape[0] == T
+    pa = _vector("advantages", advantages, T if per_row else N, torch.float32, dev)
+    if kl_coef and ref_logp is None:
+        raise ValueError("policy_loss: a KL term needs ref_logp, the reference policy's token_logp")
+    pr = _vector("ref_logp", ref_logp, T, torch.float32, dev) if ref_logp is not None else 0
+    low, high = clip
+    g, pg, ldg, tail = _gradient(dlogits, logits)
+    out = torch.empty(3 + T, dtype=torch.float32, device=dev)
+    p = out.data_ptr()
+    opts = _POLICY.pack(po, pr, pa, p, p + 12, pg, ldg, low, high, kl_coef, grad_scale, int(bool(per_row)), POLICY_REDUCTIONS[reduction], tail, 0)
+    _call("wd_policy_loss_fwd_bwd", dev, T, rows, opts)
+    return PolicyLoss(out[0], out[1], out[2], out[3:], g)
