@@ -6,6 +6,8 @@
 //   lp = (z_t - m) - ln s                                 (not z_t - lse: the difference keeps its low bits where |m| is large)
 //   dlp/dz_v = [v = t] - e^(z_v - m) / s,  dz_v = c * dlp/dz_v   with c = dloss/dlp of the row
 // Everything a row needs from other rows is a handful of numbers, so the kernels are passes over rows and HBM bounds them.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -18,6 +20,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int64_t kCountSeqs = 1024;      // up to as many sequences every wavefront adds the counts up itself
 constexpr float kLowest = -3.402823466e38f;
 
 // ---- element types: one 16-byte word <-> floats.  Sums and statistics are fp32; gradients are rounded once, to nearest even.
@@ -179,22 +182,26 @@ __device__ __forceinline__ void seq_range(const wd_seq_rows_t &q, int64_t n, int
 __device__ __forceinline__ int64_t first_row(const wd_seq_rows_t &q) { return min((int64_t)max(q.seq_offs[0], 0), q.rows); }
 __device__ __forceinline__ int64_t last_row(const wd_seq_rows_t &q) { return min((int64_t)max(q.seq_offs[q.nseq], 0), q.rows); }
 __device__ __forceinline__ bool outside(const wd_seq_rows_t &q, int64_t r) { return r < first_row(q) || r >= last_row(q); }
-template <int TH> __device__ __forceinline__ void zero_outside(const wd_seq_rows_t &q, float *v) {
-  for (int64_t r = threadIdx.x; r < first_row(q); r += TH) v[r] = 0.f;
-  for (int64_t r = last_row(q) + threadIdx.x; r < q.rows; r += TH) v[r] = 0.f;
-}
 // workgroup (part, row): parts of a row are neighbours in x, rows fill y and z (a grid dimension holds 2^32 lanes)
 __device__ __forceinline__ int64_t block_row() { return (int64_t)blockIdx.z * gridDim.y + blockIdx.y; }
 __device__ __forceinline__ bool is_action(const wd_seq_rows_t &q, int32_t t) { return t >= 0 && t < q.vocab; }
 
-// ---- (m, s) of every part of every row: workgroup (row, part)
+__device__ __forceinline__ float logp(float xt, float m, float s) { return (xt - m) - logf(s); }
+
+// ---- (m, s) of every part of every row: workgroup (row, part).  A row in one part is done here, its log-probability too.
 template <int DT>
-__global__ void __launch_bounds__(256) k_row_stats(wd_seq_rows_t q, int32_t nsplit, float2 *__restrict__ part) {
+__global__ void __launch_bounds__(256)
+k_row_stats(wd_seq_rows_t q, int32_t nsplit, float2 *__restrict__ part, float2 *__restrict__ stat, float *__restrict__ token) {
   constexpr int TH = 256, U = 4, W = Elem<DT>::W;
   __shared__ float lm[TH / kWave], ls[TH / kWave];
   const int64_t r = block_row();
   const int z = (int)blockIdx.x;
-  if (r >= q.rows || outside(q, r) || !is_action(q, q.targets[r])) return;
+  if (r >= q.rows) return;
+  const int32_t t = q.targets[r];
+  if (outside(q, r) || !is_action(q, t)) {
+    if (z == 0 && threadIdx.x == 0) token[r] = 0.f;
+    return;
+  }
   const Row<DT> row(q.logits, q.ld, r, (int)q.vocab);
   const int per = (row.nb + nsplit - 1) / nsplit;
   const int j1 = min(row.nb, (z + 1) * per);
@@ -234,68 +241,108 @@ __global__ void __launch_bounds__(256) k_row_stats(wd_seq_rows_t q, int32_t nspl
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int w = 1; w < TH / kWave; ++w) join(m, s, lm[w], ls[w]);
-    part[r * nsplit + z] = make_float2(m, s);
+    if (nsplit == 1) {
+      stat[r] = make_float2(m, s);
+      token[r] = logp(Elem<DT>::to_float(row.p[t]), m, s);
+    } else {
+      part[r * nsplit + z] = make_float2(m, s);
+    }
   }
 }
 
-// the row's parts joined, and its target's log-probability
+// the parts (a power of two, at most 64) of row r joined by as many lanes, part z in lane z of them; the first one stores (m, s) and the
+// target's log-probability and returns it
 template <int DT>
-__device__ __forceinline__ float row_logp(const wd_seq_rows_t &q, int64_t r, int32_t t, int32_t nsplit, const float2 *part, float2 &ms) {
-  ms = part[r * nsplit];
-  for (int z = 1; z < nsplit; ++z) {
-    const float2 o = part[r * nsplit + z];
-    join(ms.x, ms.y, o.x, o.y);
+__device__ __forceinline__ float row_join(const wd_seq_rows_t &q, int64_t r, int32_t t, int32_t nsplit, int z, const float2 *part, float2 *stat,
+                                          float *token) {
+  float2 ms = part[r * nsplit + z];
+  const float xt = Elem<DT>::to_float(((const typename Elem<DT>::type *)q.logits)[r * q.ld + t]);
+  for (int o = 1; o < nsplit; o <<= 1) join(ms.x, ms.y, __shfl_xor(ms.x, o), __shfl_xor(ms.y, o));
+  const float lp = logp(xt, ms.x, ms.y);
+  if (z == 0) {
+    stat[r] = ms;
+    token[r] = lp;
   }
-  const float x = Elem<DT>::to_float(((const typename Elem<DT>::type *)q.logits)[r * q.ld + t]);
-  return (x - ms.x) - logf(ms.y);
+  return lp;
 }
 
-// sum and number of the actions of rows [a, b); token_logp and the joined (m, s) of each row stored on the way
+// sum and number of the actions of rows [a, b)
 template <int DT, int TH>
-__device__ __forceinline__ void seq_logp(const wd_seq_rows_t &q, int64_t a, int64_t b, int32_t nsplit, const float2 *part, float *token,
-                                         float2 *stat, double &sum, int32_t &count, double *ld, int32_t *li) {
+__device__ __forceinline__ void seq_logp(const wd_seq_rows_t &q, int64_t a, int64_t b, int32_t nsplit, const float2 *part, float2 *stat,
+                                         float *token, double &sum, int32_t &count, double *ld, int32_t *li) {
   double v = 0.0;      // long sums in 64 bits: a sequence of a thousand items sums to thousands, its pair's difference to units
   int32_t c = 0;
-  for (int64_t r = a + threadIdx.x; r < b; r += TH) {
-    const int32_t t = q.targets[r];
-    float lp = 0.f;
-    if (is_action(q, t)) {
-      float2 ms;
-      lp = row_logp<DT>(q, r, t, nsplit, part, ms);
-      if (stat) stat[r] = ms;
-      v += lp;
-      ++c;
+  if (nsplit == 1) {
+    for (int64_t r = a + threadIdx.x; r < b; r += TH) {
+      v += token[r];      // 0 where the row is no action
+      c += is_action(q, q.targets[r]);
     }
-    if (token) token[r] = lp;
+  } else {
+    const int z = threadIdx.x & (nsplit - 1);
+    for (int64_t r = a + threadIdx.x / nsplit; r < b; r += TH / nsplit) {      // the lanes of a row leave together
+      const int32_t t = q.targets[r];
+      if (!is_action(q, t)) continue;
+      const float lp = row_join<DT>(q, r, t, nsplit, z, part, stat, token);
+      if (z == 0) {
+        v += lp;
+        ++c;
+      }
+    }
   }
   sum = block_sum<TH>(v, ld);
   count = block_sum<TH>(c, li);
 }
 
-// ---- scores: workgroup n = sequence n; one more zeroes token_logp behind the last sequence
+// ---- scores: workgroup n = sequence n
 template <int DT>
 __global__ void __launch_bounds__(256)
-k_seq_logp(wd_seq_rows_t q, int32_t nsplit, int32_t length_norm, const float2 *__restrict__ part, float *__restrict__ token,
-           float *__restrict__ seq) {
+k_seq_logp(wd_seq_rows_t q, int32_t nsplit, int32_t length_norm, const float2 *__restrict__ part, float2 *__restrict__ stat,
+           float *__restrict__ token, float *__restrict__ seq) {
   constexpr int TH = 256;
   __shared__ double ld[TH / kWave];
   __shared__ int32_t li[TH / kWave];
   const int64_t n = block_row();
-  if (n == q.nseq) zero_outside<TH>(q, token);
   if (n >= q.nseq) return;
   int64_t a, b;
   seq_range(q, n, a, b);
   double sum;
   int32_t count;
-  seq_logp<DT, TH>(q, a, b, nsplit, part, token, nullptr, sum, count, ld, li);
+  seq_logp<DT, TH>(q, a, b, nsplit, part, stat, token, sum, count, ld, li);
   if (threadIdx.x == 0) seq[n] = (float)(length_norm ? sum / max(count, 1) : sum);
 }
 
 // log sigma(h) without overflow on either side
 __device__ __forceinline__ double log_sigmoid(double h) { return fmin(h, 0.0) - log1p(exp(-fabs(h))); }
 
-// ---- pairs: workgroup i = sequences 2i (chosen) and 2i + 1 (rejected); leaves dloss/dlp of every row.  The scalars of a pair are
-// computed in 64 bits: there are a few of them, and the coefficient multiplies whole rows.
+// ---- pairs.  The scalars of a pair are computed in 64 bits: there are a few of them, and the coefficient multiplies whole rows.
+__device__ __forceinline__ double pair_difference(const wd_pref_t &o, int64_t i, double chosen, double rejected) {
+  return chosen - rejected - (o.ref_logp ? (double)o.ref_logp[2 * i] - (double)o.ref_logp[2 * i + 1] : 0.0);
+}
+__device__ __forceinline__ double pair_loss_of(const wd_pref_t &o, double d) {
+  if (o.kind == WD_PREF_SQUARE) {
+    const double h = d - 0.5 / (double)o.beta;
+    return h * h;
+  }
+  const double h = (double)o.beta * d - (double)o.margin, eps = (double)o.label_smoothing;
+  return -(1.0 - eps) * log_sigmoid(h) - eps * log_sigmoid(-h);
+}
+// grad_scale times dloss/dd of the batch's loss
+__device__ __forceinline__ double pair_slope(const wd_pref_t &o, int64_t i, double d) {
+  const double w = (double)o.scale * (o.weights ? (double)o.weights[i] : 1.0) * (double)o.grad_scale;
+  if (o.kind == WD_PREF_SQUARE) return 2.0 * (d - 0.5 / (double)o.beta) * w;
+  // sigma(h) - (1 - eps) as eps sigma(h) - (1 - eps) sigma(-h): no cancellation where the pair is settled
+  const double h = (double)o.beta * d - (double)o.margin, eps = (double)o.label_smoothing;
+  const double e = exp(-fabs(h)), big = 1.0 / (1.0 + e), small = e * big;
+  return (double)o.beta * w * (eps * (h >= 0 ? big : small) - (1.0 - eps) * (h >= 0 ? small : big));
+}
+__device__ __forceinline__ void store_pair(const wd_pref_t &o, int64_t i, double d, double loss, const double *lp) {
+  o.pair_loss[i] = (float)loss;
+  o.difference[i] = (float)d;
+  o.seq_logp[2 * i] = (float)lp[0];
+  o.seq_logp[2 * i + 1] = (float)lp[1];
+}
+
+// workgroup i = pair i; leaves dloss/dlp of every row
 template <int DT>
 __global__ void __launch_bounds__(256)
 k_pref_pairs(wd_seq_rows_t q, wd_pref_t o, int32_t nsplit, const float2 *__restrict__ part, float2 *__restrict__ stat,
@@ -304,48 +351,39 @@ k_pref_pairs(wd_seq_rows_t q, wd_pref_t o, int32_t nsplit, const float2 *__restr
   __shared__ double ld[TH / kWave];
   __shared__ int32_t li[TH / kWave];
   const int64_t i = block_row();
-  if (i == q.nseq / 2) zero_outside<TH>(q, o.token_logp);
   if (i >= q.nseq / 2) return;
   int64_t a[2], b[2];
   double lp[2];
   int32_t n[2];
   for (int k = 0; k < 2; ++k) {
     seq_range(q, 2 * i + k, a[k], b[k]);
-    seq_logp<DT, TH>(q, a[k], b[k], nsplit, part, o.token_logp, stat, lp[k], n[k], ld, li);
+    seq_logp<DT, TH>(q, a[k], b[k], nsplit, part, stat, o.token_logp, lp[k], n[k], ld, li);
     n[k] = o.length_norm ? max(n[k], 1) : 1;
     lp[k] /= n[k];
   }
-  double d = lp[0] - lp[1];
-  if (o.ref_logp) d -= (double)o.ref_logp[2 * i] - (double)o.ref_logp[2 * i + 1];
-  const double w = (double)o.scale * (o.weights ? (double)o.weights[i] : 1.0);
-  double loss, slope;
-  if (o.kind == WD_PREF_LOGISTIC) {
-    const double h = (double)o.beta * d - (double)o.margin, eps = (double)o.label_smoothing;
-    loss = -(1.0 - eps) * log_sigmoid(h) - eps * log_sigmoid(-h);
-    // dloss/dh = sigma(h) - (1 - eps), as eps sigma(h) - (1 - eps) sigma(-h): no cancellation where the pair is settled
-    const double e = exp(-fabs(h)), big = 1.0 / (1.0 + e), small = e / (1.0 + e);
-    slope = (double)o.beta * (eps * (h >= 0 ? big : small) - (1.0 - eps) * (h >= 0 ? small : big));
-  } else {
-    const double h = d - 0.5 / (double)o.beta;
-    loss = h * h;
-    slope = 2.0 * h;
-  }
-  if (threadIdx.x == 0) {
-    o.pair_loss[i] = (float)loss;
-    o.difference[i] = (float)d;
-    o.seq_logp[2 * i] = (float)lp[0];
-    o.seq_logp[2 * i + 1] = (float)lp[1];
-  }
+  const double d = pair_difference(o, i, lp[0], lp[1]), slope = pair_slope(o, i, d);
+  if (threadIdx.x == 0) store_pair(o, i, d, pair_loss_of(o, d), lp);
   for (int k = 0; k < 2; ++k) {
-    const float c = (float)((k ? -slope : slope) * w * (double)o.grad_scale / n[k]);
+    const float c = (float)((k ? -slope : slope) / n[k]);
     for (int64_t r = a[k] + threadIdx.x; r < b[k]; r += TH) coef[r] = c;
   }
 }
 
 // ---- gradient of the logits from (m, s, coefficient) of each row: workgroup (row, part); the last one adds the loss up
 template <int TH> __device__ __forceinline__ void weighted_sum(const float *v, const float *w, int64_t n, double scale, float *out, double *ld) {
+  constexpr int U = 8;
   double t = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += TH) t += (double)v[i] * (w ? (double)w[i] : 1.0);
+  for (int64_t i = threadIdx.x; i < n; i += TH * U) {
+    float x[U], y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = i + u * TH < n;
+      x[u] = in ? v[i + u * TH] : 0.f;
+      y[u] = in && w ? w[i + u * TH] : 1.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) t += (double)x[u] * (double)y[u];
+  }
   t = block_sum<TH>(t, ld);
   if (threadIdx.x == 0) *out = (float)(t * scale);
 }
@@ -415,37 +453,109 @@ k_logits_grad(wd_seq_rows_t q, void *dlogits, int64_t ldg, int32_t zero_tail, in
   grad_part<DT, TH>(row, (typename Elem<DT>::type *)dlogits + r * ldg, z, nsplit, action, t, ms.x, ms.y, action ? coef[r] : 0.f);
 }
 
-// ---- clipped policy loss
-// weights of the rows (sum | mean over actions | mean over sequences of means) and the advantages by row
-template <int TH>
-__global__ void __launch_bounds__(TH) k_policy_rows(wd_seq_rows_t q, wd_policy_t o, float *__restrict__ w, float *__restrict__ adv) {
-  __shared__ int32_t li[TH / kWave];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-  int32_t actions = 0, seqs = 0;
-  // a wavefront per sequence counts its actions; one workgroup, so the totals need no second launch
-  for (int64_t n = wave; n < q.nseq; n += TH / kWave) {
+// sequence of row r, by a wavefront: the number of sequences that end in front of it
+__device__ __forceinline__ int64_t wave_sequence(const wd_seq_rows_t &q, int64_t r) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int64_t s = 0;
+  for (int64_t k = lane; k - lane < q.nseq; k += kWave) s += __popcll(__ballot(k < q.nseq && q.seq_offs[k + 1] <= r));
+  return s;
+}
+
+// small batches: pairs and gradient in one launch.  Every wavefront adds its row's pair up for itself (rows in one part, their
+// log-probabilities are there); the workgroup behind the last row does the pairs' outputs and the loss.
+__device__ __forceinline__ void wave_pair(const wd_seq_rows_t &q, const wd_pref_t &o, int64_t i, double *lp, int32_t *n) {
+  const int lane = threadIdx.x & (kWave - 1);
+  for (int k = 0; k < 2; ++k) {
     int64_t a, b;
-    seq_range(q, n, a, b);
+    seq_range(q, 2 * i + k, a, b);
+    double v = 0.0;
     int32_t c = 0;
-    for (int64_t r = a + lane; r < b; r += kWave) c += is_action(q, q.targets[r]);
-    c = wave_sum(c);
-    const float inv = o.reduction == WD_POLICY_SEQUENCE_MEAN ? 1.0f / (float)max(c, 1) : 1.0f;
-    const float av = o.adv_per_row ? 0.f : o.advantages[n];
     for (int64_t r = a + lane; r < b; r += kWave) {
-      w[r] = inv;
-      adv[r] = o.adv_per_row ? o.advantages[r] : av;
+      v += o.token_logp[r];
+      c += is_action(q, q.targets[r]);
     }
-    if (lane == 0) {
-      actions += c;
-      seqs += c > 0;
+    n[k] = 1;
+    if (o.length_norm) n[k] = max(wave_sum(c), 1);
+    lp[k] = wave_sum(v) / n[k];
+  }
+}
+template <int DT>
+__global__ void __launch_bounds__(256) k_pref_grad(wd_seq_rows_t q, wd_pref_t o, int32_t nsplit, const float2 *__restrict__ stat) {
+  constexpr int TH = 256;
+  __shared__ double ld[TH / kWave];
+  const int64_t r = block_row();
+  const int z = (int)blockIdx.x, lane = threadIdx.x & (kWave - 1);
+  double lp[2];
+  int32_t n[2];
+  if (r == q.rows && z == 0) {
+    double total = 0.0;
+    for (int64_t i = threadIdx.x / kWave; i < q.nseq / 2; i += TH / kWave) {
+      wave_pair(q, o, i, lp, n);
+      const double d = pair_difference(o, i, lp[0], lp[1]), loss = pair_loss_of(o, d);
+      if (lane == 0) {
+        store_pair(o, i, d, loss, lp);
+        total += loss * (o.weights ? (double)o.weights[i] : 1.0);
+      }
     }
+    total = block_sum<TH>(total, ld);
+    if (threadIdx.x == 0) *o.loss = (float)(total * (double)o.scale);
   }
-  actions = block_sum<TH>(actions, li);
-  seqs = block_sum<TH>(seqs, li);
-  if (threadIdx.x == 0) {
-    const int32_t d = o.reduction == WD_POLICY_TOKEN_MEAN ? actions : o.reduction == WD_POLICY_SEQUENCE_MEAN ? seqs : 1;
-    w[q.rows] = 1.0f / (float)max(d, 1);
+  if (r >= q.rows || !o.dlogits) return;
+  const bool tail = outside(q, r);
+  if (tail && !o.zero_tail) return;
+  const int32_t t = q.targets[r];
+  const bool action = !tail && is_action(q, t);
+  const Row<DT> row(q.logits, q.ld, r, (int)q.vocab);
+  float2 ms = make_float2(0.f, 1.f);
+  float c = 0.f;
+  if (action) {
+    ms = stat[r];
+    const int64_t s = wave_sequence(q, r);
+    wave_pair(q, o, s / 2, lp, n);
+    const double slope = pair_slope(o, s / 2, pair_difference(o, s / 2, lp[0], lp[1]));
+    c = (float)(s & 1 ? -slope / n[1] : slope / n[0]);
   }
+  grad_part<DT, TH>(row, (typename Elem<DT>::type *)o.dlogits + r * o.ld_dlogits, z, nsplit, action, t, ms.x, ms.y, c);
+}
+
+// ---- clipped policy loss
+// workgroup n = sequence n: its number of actions, and by row the part of the weight that is the sequence's own and the advantage
+template <int TH>
+__global__ void __launch_bounds__(TH)
+k_policy_rows(wd_seq_rows_t q, wd_policy_t o, float *__restrict__ w, float *__restrict__ adv, int32_t *__restrict__ cnt) {
+  __shared__ int32_t li[TH / kWave];
+  const int64_t n = block_row();
+  if (n >= q.nseq) return;
+  int64_t a, b;
+  seq_range(q, n, a, b);
+  int32_t c = 0;
+  for (int64_t r = a + threadIdx.x; r < b; r += TH) c += is_action(q, q.targets[r]);
+  c = block_sum<TH>(c, li);
+  const float inv = o.reduction == WD_POLICY_SEQUENCE_MEAN ? 1.0f / (float)max(c, 1) : 1.0f;
+  const float av = o.adv_per_row ? 0.f : o.advantages[n];
+  for (int64_t r = a + threadIdx.x; r < b; r += TH) {
+    w[r] = inv;
+    adv[r] = o.adv_per_row ? o.advantages[r] : av;
+  }
+  if (threadIdx.x == 0) cnt[n] = c;
+}
+// the rest of every weight, the same in all rows: 1, 1 / actions, or 1 / sequences with an action; `lane` of `step` lanes adds
+__device__ __forceinline__ int32_t policy_count(const wd_seq_rows_t &q, const wd_policy_t &o, const int32_t *cnt, int lane, int step) {
+  int32_t d = 0;
+  if (o.reduction != WD_POLICY_SUM)
+    for (int64_t n = lane; n < q.nseq; n += step) d += o.reduction == WD_POLICY_TOKEN_MEAN ? cnt[n] : cnt[n] > 0;
+  return d;
+}
+__global__ void __launch_bounds__(1024) k_policy_total(wd_seq_rows_t q, wd_policy_t o, int32_t *__restrict__ cnt) {
+  __shared__ int32_t li[1024 / kWave];
+  const int32_t d = block_sum<1024>(policy_count(q, o, cnt, threadIdx.x, 1024), li);
+  if (threadIdx.x == 0) cnt[q.nseq] = d;
+}
+// by a wavefront; many sequences: k_policy_total has done it
+__device__ __forceinline__ float policy_factor(const wd_seq_rows_t &q, const wd_policy_t &o, const int32_t *cnt) {
+  if (o.reduction == WD_POLICY_SUM) return 1.f;
+  const int32_t d = q.nseq > kCountSeqs ? cnt[q.nseq] : wave_sum(policy_count(q, o, cnt, threadIdx.x & (kWave - 1), kWave));
+  return 1.0f / (float)max(d, 1);
 }
 
 struct PolicyRow {
@@ -472,9 +582,11 @@ __device__ __forceinline__ PolicyRow policy_row(const wd_policy_t &o, float lp, 
 }
 
 // the whole row in registers between its statistics and its gradient: one read and one write of the logits, workgroup = row
+// w == nullptr: no launch has made weights and advantages; each wavefront finds them (no mean over sequences)
 template <int DT, int TH, int NV>
-__global__ void __launch_bounds__(TH)
-k_policy_resident(wd_seq_rows_t q, wd_policy_t o, const float *__restrict__ w, const float *__restrict__ adv, float *__restrict__ rows3) {
+__global__ void __launch_bounds__(TH, TH == 512 ? 4 : 1)
+k_policy_resident(wd_seq_rows_t q, wd_policy_t o, const float *__restrict__ w, const float *__restrict__ adv,
+                  const int32_t *__restrict__ cnt, float *__restrict__ rows3) {
   constexpr int W = Elem<DT>::W;
   typedef typename Elem<DT>::type type;
   __shared__ float lf[TH / kWave], lg[TH / kWave];
@@ -506,7 +618,20 @@ k_policy_resident(wd_seq_rows_t q, wd_policy_t o, const float *__restrict__ w, c
   const int e = row.edge(threadIdx.x);
   const float xe = e >= 0 ? Elem<DT>::to_float(row.p[e]) : -INFINITY;
   const float xt = Elem<DT>::to_float(row.p[t]);
-  const float wr = w[r] * w[q.rows], ar = adv[r], old = o.old_logp[r], ref = o.ref_logp ? o.ref_logp[r] : 0.f;
+  const float old = o.old_logp[r], ref = o.ref_logp ? o.ref_logp[r] : 0.f;
+  float wr = 1.f, ar;
+  if (w) {
+    wr = w[r] * policy_factor(q, o, cnt);
+    ar = adv[r];
+  } else {
+    ar = o.advantages[o.adv_per_row ? r : wave_sequence(q, r)];
+    if (o.reduction == WD_POLICY_TOKEN_MEAN) {
+      int32_t c = 0;
+      const int64_t end = last_row(q);
+      for (int64_t i = first_row(q) + (threadIdx.x & (kWave - 1)); i < end; i += kWave) c += is_action(q, q.targets[i]);
+      wr = 1.0f / (float)wave_sum(c);
+    }
+  }
   hold(v);
   float x[W], m = fmaxf(kLowest, xe);
 #pragma unroll
@@ -525,7 +650,7 @@ k_policy_resident(wd_seq_rows_t q, wd_policy_t o, const float *__restrict__ w, c
     for (int i = 0; i < W; ++i) s += exp_rel(x[i], m);
   }
   s = block_sum<TH>(s, lg);
-  const float lp = (xt - m) - logf(s);
+  const float lp = logp(xt, m, s);
   const PolicyRow p = policy_row(o, lp, old, ar, ref);
   if (threadIdx.x == 0) {
     o.token_logp[r] = lp;
@@ -555,26 +680,26 @@ k_policy_resident(wd_seq_rows_t q, wd_policy_t o, const float *__restrict__ w, c
   }
 }
 
-// rows whose statistics came in parts: loss and coefficient of each row, a lane per row
+// rows too long for the registers: loss and coefficient of each row, a lane per part of it
 template <int DT>
 __global__ void __launch_bounds__(256)
 k_policy_join(wd_seq_rows_t q, wd_policy_t o, int32_t nsplit, const float2 *__restrict__ part, const float *__restrict__ w,
-              const float *__restrict__ adv, float2 *__restrict__ stat, float *__restrict__ coef, float *__restrict__ rows3) {
-  const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+              const float *__restrict__ adv, const int32_t *__restrict__ cnt, float2 *__restrict__ stat, float *__restrict__ coef, float *__restrict__ rows3) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, r = i / nsplit;
+  const int z = (int)(i & (nsplit - 1));
+  const float factor = policy_factor(q, o, cnt);      // whole wavefronts
   if (r >= q.rows) return;
   float lp = 0.f, wr = 0.f, c = 0.f;
   PolicyRow p = {0.f, 0.f, 0.f, 0.f};
   const int32_t t = q.targets[r];
   if (!outside(q, r) && is_action(q, t)) {
-    float2 ms;
-    lp = row_logp<DT>(q, r, t, nsplit, part, ms);
-    stat[r] = ms;
-    wr = w[r] * w[q.rows];
+    lp = nsplit == 1 ? o.token_logp[r] : row_join<DT>(q, r, t, nsplit, z, part, stat, o.token_logp);
+    wr = w[r] * factor;
     p = policy_row(o, lp, o.old_logp[r], adv[r], o.ref_logp ? o.ref_logp[r] : 0.f);
     c = p.slope * wr * o.grad_scale;
   }
+  if (z) return;
   coef[r] = c;
-  o.token_logp[r] = lp;
   rows3[r] = p.loss * wr;
   rows3[q.rows + r] = p.kl * wr;
   rows3[2 * q.rows + r] = p.clipped * wr;
@@ -601,23 +726,29 @@ int check_rows(const char *who, const wd_seq_rows_t *q) {
 
 int words(const wd_seq_rows_t &q) { return (int)(q.vocab / (q.dtype == WD_T_F32 ? 4 : 8)); }      // whole words of a row, at most
 
-// parts of a row: enough workgroups for every CU where there are few rows, at least 4 KB each
+// parts of a row: two workgroups for every CU where there are few rows, at least 4 KB each; a power of two up to a wavefront of them
 int row_split(const wd_seq_rows_t &q) {
-  if (q.rows < 1) return 1;
-  const int64_t want = ceil_div(1024, q.rows), most = words(q) / 256;
-  return (int)(want < 1 || most < 1 ? 1 : want < most ? want : most);
+  int n = 1;
+  while (n < kWave && q.rows * n < 2 * kCUs && words(q) >= 512 * n) n *= 2;
+  return n;
 }
 // parts of a row for the gradient pass, 16 KB each: a lane has four words in flight
 int grad_split(const wd_seq_rows_t &q) { return words(q) <= 1024 ? 1 : (int)ceil_div(words(q), 1024); }
+
+// batches whose rows find their pair, weight or advantage themselves instead of in a launch of its own
+constexpr int64_t kSelfRows = 256, kSelfSeqs = 256;
+// whole words of the longest row that a workgroup holds in registers: 1024 lanes x 16
+constexpr int kResidentWords = 16384;
 
 dim3 row_grid(int64_t rows, int parts) {
   const int64_t y = rows < 32768 ? rows : 32768;
   return dim3((unsigned)parts, (unsigned)y, (unsigned)ceil_div(rows, y));
 }
 
-struct Work {      // [rows * nsplit] (m, s) parts | [rows] (m, s) | [rows] coefficients | 3 [rows] | [rows + 1] weights | [rows] advantages
+struct Work {      // [rows * nsplit] (m, s) parts | [rows] (m, s) | [rows] coefficients | 3 [rows] | [rows] weights | [rows] advantages | counts
   float2 *part, *stat;
   float *coef, *rows3, *w, *adv;
+  int32_t *cnt;
   Work(const wd_seq_rows_t &q, float *p) {
     const int64_t T = q.rows;
     part = (float2 *)p;
@@ -625,7 +756,8 @@ struct Work {      // [rows * nsplit] (m, s) parts | [rows] (m, s) | [rows] coef
     coef = (float *)(stat + T);
     rows3 = coef + T;
     w = rows3 + 3 * T;
-    adv = w + T + 1;
+    adv = w + T;
+    cnt = (int32_t *)(adv + T);
   }
 };
 
@@ -635,9 +767,33 @@ template <typename F> void by_type(int32_t dtype, F f) {
   else f(std::integral_constant<int, WD_T_BF16>());
 }
 
-void launch_stats(const wd_seq_rows_t &q, int nsplit, float2 *part, hipStream_t st) {
+void launch_stats(const wd_seq_rows_t &q, int nsplit, const Work &k, float *token, hipStream_t st) {
   if (q.rows < 1) return;
-  by_type(q.dtype, [&](auto dt) { k_row_stats<decltype(dt)::value><<<row_grid(q.rows, nsplit), 256, 0, st>>>(q, nsplit, part); });
+  by_type(q.dtype, [&](auto dt) { k_row_stats<decltype(dt)::value><<<row_grid(q.rows, nsplit), 256, 0, st>>>(q, nsplit, k.part, k.stat, token); });
+}
+
+// A row in the registers of a workgroup, NV words a lane.  Two or more workgroups have to fit on a CU, so that one loads or stores while
+// another adds up, and no lane should hold many words it has not got: measured on bf16 rows, 0.8 GB in and out, TB/s:
+//   words 125 (0.4 GB)  64 x 2 2.84, 128 x 1 2.25, 256 x 1 1.56      250   128 x 2 3.77, 64 x 4 3.70, 256 x 1 2.78
+//   1000  512 x 2 4.76, 256 x 4 4.57, 1024 x 1 3.11     2000  512 x 4 5.14, 256 x 8 4.89, 1024 x 2 4.68
+//   4000  1024 x 4 5.28, 512 x 8 4.97, 256 x 16 4.89    8000  512 x 16 4.94, 256 x 32 4.79, 1024 x 8 4.15
+//   12500 512 x 25 4.49 (128 registers), 4.22 (151), 1024 x 13 4.12        16375 1024 x 16 4.08, 512 x 32 3.99
+template <int DT, int TH, int... NV>
+bool launch_resident_of(int nw, const wd_seq_rows_t &q, const wd_policy_t &o, const Work &k, hipStream_t st) {
+  bool done = false;
+  ((done || nw > TH * NV ? (void)0
+                         : (k_policy_resident<DT, TH, NV><<<row_grid(q.rows, 1), TH, 0, st>>>(q, o, k.w, k.adv, k.cnt, k.rows3), (void)(done = true))),
+   ...);
+  return done;
+}
+template <int DT> bool launch_resident(const wd_seq_rows_t &q, const wd_policy_t &o, const Work &k, hipStream_t st) {
+  const int nw = words(q);
+  if (nw <= 128) return launch_resident_of<DT, 64, 1, 2>(nw, q, o, k, st);
+  if (nw <= 512) return launch_resident_of<DT, 128, 2, 3, 4>(nw, q, o, k, st);
+  if (nw <= 2048) return launch_resident_of<DT, 512, 2, 3, 4>(nw, q, o, k, st);
+  if (nw <= 4096) return launch_resident_of<DT, 1024, 3, 4>(nw, q, o, k, st);
+  if (nw <= 12800) return launch_resident_of<DT, 512, 9, 10, 11, 12, 13, 14, 16, 18, 20, 22, 25>(nw, q, o, k, st);
+  return nw <= kResidentWords && launch_resident_of<DT, 1024, 14, 16>(nw, q, o, k, st);
 }
 
 }  // namespace
@@ -645,7 +801,7 @@ void launch_stats(const wd_seq_rows_t &q, int nsplit, float2 *part, hipStream_t 
 extern "C" int64_t wd_policy_workspace_floats(const wd_seq_rows_t *rows) {
   const int rc = check_rows(__func__, rows);
   if (rc) return rc;
-  return rows->rows * (2 * (int64_t)row_split(*rows) + 2 + 1 + 3 + 1 + 1) + 1;
+  return rows->rows * (2 * (int64_t)row_split(*rows) + 2 + 1 + 3 + 1 + 1) + rows->nseq + 1;
 }
 
 extern "C" int wd_seq_logp(const wd_seq_rows_t *rows, int32_t length_norm, float *token_logp, float *seq_logp, float *ws,
@@ -656,9 +812,9 @@ extern "C" int wd_seq_logp(const wd_seq_rows_t *rows, int32_t length_norm, float
   hipStream_t st = as_stream(stream);
   const Work k(q, ws);
   const int ns = row_split(q);
-  launch_stats(q, ns, k.part, st);
-  by_type(q.dtype, [&](auto dt) {
-    k_seq_logp<decltype(dt)::value><<<row_grid(q.nseq + 1, 1), 256, 0, st>>>(q, ns, length_norm, k.part, token_logp, seq_logp);
+  launch_stats(q, ns, k, token_logp, st);
+  if (q.nseq > 0) by_type(q.dtype, [&](auto dt) {
+    k_seq_logp<decltype(dt)::value><<<row_grid(q.nseq, 1), 256, 0, st>>>(q, ns, length_norm, k.part, k.stat, token_logp, seq_logp);
   });
   return check_launch(__func__);
 }
@@ -679,14 +835,18 @@ extern "C" int wd_pref_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_pref_t *
   hipStream_t st = as_stream(stream);
   const Work k(q, ws);
   const int ns = row_split(q), gs = grad_split(q);
-  launch_stats(q, ns, k.part, st);
+  launch_stats(q, ns, k, o.token_logp, st);
   wd_seq_rows_t last = q;
   if (!o.dlogits) last.rows = 0;      // the loss alone
   by_type(q.dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    k_pref_pairs<DT><<<row_grid(q.nseq / 2 + 1, 1), 256, 0, st>>>(q, o, ns, k.part, k.stat, k.coef);
-    k_logits_grad<DT><<<row_grid(last.rows + 1, gs), 256, 0, st>>>(last, o.dlogits, o.ld_dlogits, o.zero_tail, gs, k.stat, k.coef,
-                                                                            o.pair_loss, o.weights, (double)o.scale, o.loss);
+    if (ns == 1 && q.rows <= kSelfRows && q.nseq <= kSelfSeqs) {
+      k_pref_grad<DT><<<row_grid(q.rows + 1, gs), 256, 0, st>>>(q, o, gs, k.stat);
+      return;
+    }
+    if (q.nseq > 0) k_pref_pairs<DT><<<row_grid(q.nseq / 2, 1), 256, 0, st>>>(q, o, ns, k.part, k.stat, k.coef);
+    k_logits_grad<DT><<<row_grid(last.rows + 1, gs), 256, 0, st>>>(last, o.dlogits, o.ld_dlogits, o.zero_tail, gs, k.stat, k.coef, o.pair_loss,
+                                                                   o.weights, (double)o.scale, o.loss);
   });
   return check_launch(__func__);
 }
@@ -703,21 +863,21 @@ extern "C" int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy
   WD_REQUIRE(!o.dlogits || o.ld_dlogits >= q.vocab, "row stride of the gradient below the row length");
   WD_REQUIRE((uintptr_t)o.dlogits % (q.dtype == WD_T_F32 ? 4 : 2) == 0, "gradient not aligned to its element size");
   hipStream_t st = as_stream(stream);
-  const Work k(q, ws);
-  k_policy_rows<1024><<<1, 1024, 0, st>>>(q, o, k.w, k.adv);
+  Work k(q, ws);
   const int nw = words(q);
+  if (nw <= kResidentWords && q.rows <= kSelfRows && q.nseq <= kSelfSeqs && o.reduction != WD_POLICY_SEQUENCE_MEAN) k.w = nullptr;
+  else if (q.nseq > 0) {
+    if (q.rows < 256 * q.nseq) k_policy_rows<256><<<row_grid(q.nseq, 1), 256, 0, st>>>(q, o, k.w, k.adv, k.cnt);
+    else k_policy_rows<1024><<<row_grid(q.nseq, 1), 1024, 0, st>>>(q, o, k.w, k.adv, k.cnt);
+    if (q.nseq > kCountSeqs && o.reduction != WD_POLICY_SUM) k_policy_total<<<1, 1024, 0, st>>>(q, o, k.cnt);
+  }
   if (q.rows > 0) {
     by_type(q.dtype, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
-      const dim3 grid = row_grid(q.rows, 1);
-      if (nw <= 256) k_policy_resident<DT, 256, 1><<<grid, 256, 0, st>>>(q, o, k.w, k.adv, k.rows3);
-      else if (nw <= 1024) k_policy_resident<DT, 256, 4><<<grid, 256, 0, st>>>(q, o, k.w, k.adv, k.rows3);
-      else if (nw <= 4096) k_policy_resident<DT, 512, 8><<<grid, 512, 0, st>>>(q, o, k.w, k.adv, k.rows3);
-      else if (nw <= 16384) k_policy_resident<DT, 1024, 16><<<grid, 1024, 0, st>>>(q, o, k.w, k.adv, k.rows3);
-      else {
+      if (!launch_resident<DT>(q, o, k, st)) {
         const int ns = row_split(q), gs = grad_split(q);
-        launch_stats(q, ns, k.part, st);
-        k_policy_join<DT><<<dim3((unsigned)ceil_div(q.rows, 256)), 256, 0, st>>>(q, o, ns, k.part, k.w, k.adv, k.stat, k.coef, k.rows3);
+        launch_stats(q, ns, k, o.token_logp, st);
+        k_policy_join<DT><<<dim3((unsigned)ceil_div(q.rows * ns, 256)), 256, 0, st>>>(q, o, ns, k.part, k.w, k.adv, k.cnt, k.stat, k.coef, k.rows3);
         if (o.dlogits)
           k_logits_grad<DT><<<row_grid(q.rows, gs), 256, 0, st>>>(q, o.dlogits, o.ld_dlogits, o.zero_tail, gs, k.stat, k.coef, nullptr,
                                                                            nullptr, 0.0, nullptr);

@@ -88,6 +88,8 @@ class AdamW:
             self.m_scale, self.r_scale = torch.full((n // BLOCK,), 27, **u8), torch.full((n // BLOCK,), 27, **u8)
             second, scales = self.r, (self.m_scale.data_ptr(), self.r_scale.data_ptr())
         self._state = torch.zeros(8, dtype=torch.int32, device=dev)      # wd_adamw_state_t
+        #: global norm of the gradients of the last step with max_norm, before clipping; the next step writes it
+        self.grad_norm = self._state[6:7].view(torch.float32)[0]
         self._partials = torch.zeros(PARTIALS, dtype=torch.float64, device=dev) if max_norm is not None else None
         self._device = dev
         self._head = (self._tensors.data_ptr(), self._chunks.data_ptr(), len(chunks), self.m.data_ptr(), second.data_ptr(), *scales,
@@ -100,7 +102,7 @@ class AdamW:
         if torch.cuda.current_device() != self._device.index:
             with torch.cuda.device(self._device):
                 return self._call(name, *args)
-        return capi.call(name, *args, torch.cuda.current_stream(self._device).cuda_stream)
+        return capi.call(name, *args, torch._C._cuda_getCurrentRawStream(self._device.index))
 
     def step(self, lr=None):
         """One step on the gradients as they stand.  lr: a number, or a one-element fp32 tensor on the GPU whose value at the time of the
@@ -125,11 +127,6 @@ class AdamW:
     def skipped(self):
         """Steps skipped for a norm that was not finite (read back from the device)."""
         return int(self._state[2])
-
-    @property
-    def grad_norm(self):
-        """Global norm of the gradients of the last step with max_norm, before clipping: a one-element view that the next step writes."""
-        return self._state[6:7].view(torch.float32)
 
     def moments(self, dtype=torch.bfloat16):
         """8-bit moments as numbers: flat (m, r), r the root of the second moment; bf16 holds every value exactly."""

@@ -10,6 +10,7 @@ Layout of a batch: `logits` [rows, vocab] (fp32, fp16 or bf16; rows may be strid
 workspace come from torch's caching allocator on the current stream: calls on several streams share nothing.  Every tensor has to be
 ready on the current stream; one that another stream uses later is the caller's to record there.
 """
+import functools
 import struct
 from collections import namedtuple
 
@@ -31,7 +32,7 @@ PolicyLoss = namedtuple("PolicyLoss", "loss kl clipped token_logp dlogits")
 
 
 def _vector(name, t, n, dtype, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device != device or (n > 1 and t.stride(0) != 1):
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != 1 or t.numel() != n or t.device != device or not t.is_contiguous():
         raise ValueError("%s: a contiguous %s tensor of %d values on %s is wanted, got %s" % (name, dtype, n, device, _what(t)))
     return t.data_ptr()
 
@@ -45,18 +46,29 @@ def _rows(logits, targets, seq_offs):
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _DTYPES:
         raise ValueError("logits: a [rows, vocab] tensor of fp32, fp16 or bf16 is wanted, got %s" % _what(logits))
     T, V = logits.shape
-    if V < 1 or (T and V > 1 and logits.stride(1) != 1) or (T > 1 and logits.stride(0) < V):
-        raise ValueError("logits: at least one item, items contiguous, rows not overlapping are wanted, got %s with strides %s" % (_what(logits), logits.stride()))
-    if not logits.is_cuda:
-        raise capi.WdError("policy heads need a GPU (MI355X / gfx950); there is no CPU fallback: logits are on %s" % logits.device)
+    ld = V
+    if not logits.is_contiguous() or V < 1:
+        step, item = logits.stride()
+        if V < 1 or (T and V > 1 and item != 1) or (T > 1 and step < V):
+            raise ValueError("logits: at least one item, items contiguous, rows not overlapping are wanted, got %s with strides %s" % (_what(logits), logits.stride()))
+        ld = step if T > 1 else V
     dev = logits.device
+    if dev.type != "cuda":
+        raise capi.WdError("policy heads need a GPU (MI355X / gfx950); there is no CPU fallback: logits are on %s" % dev)
     pt = _vector("targets", targets, T, torch.int32, dev)
-    if not isinstance(seq_offs, torch.Tensor) or seq_offs.dim() != 1 or seq_offs.shape[0] < 1:
-        raise ValueError("seq_offs: an int32 tensor of sequences + 1 offsets is wanted, got %s" % _what(seq_offs))
-    N = seq_offs.shape[0] - 1
-    po = _vector("seq_offs", seq_offs, N + 1, torch.int32, dev)
-    ld = logits.stride(0) if T > 1 else V
-    return _ROWS.pack(logits.data_ptr(), ld, T, V, pt, po, N, _DTYPES[logits.dtype], 0), T, V, N, dev
+    N = seq_offs.numel() - 1 if isinstance(seq_offs, torch.Tensor) else 0
+    po = _vector("seq_offs", seq_offs, max(N, 0) + 1, torch.int32, dev)
+    code = _DTYPES[logits.dtype]
+    return _ROWS.pack(logits.data_ptr(), ld, T, V, pt, po, N, code, 0), T, V, N, dev, code
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(T, V, N, dtype):
+    """Floats of workspace, by the sizes alone."""
+    n = capi.call("wd_policy_workspace_floats", _ROWS.pack(16, V, T, V, 16, 16, N, dtype, 0))
+    if n < 0:
+        raise capi.WdError("wd_policy_workspace_floats failed (%d): %s" % (n, capi.load().wd_last_error().decode()))
+    return n + (n & 1)
 
 
 def _gradient(dlogits, logits):
@@ -74,26 +86,24 @@ def _gradient(dlogits, logits):
     return dlogits, dlogits.data_ptr(), dlogits.stride(0) if T > 1 else V, 0
 
 
-def _call(name, dev, T, rows, *args):
-    """One entry of the C ABI on the current stream of `dev`, its workspace the last argument but the stream."""
+def _call(name, dev, *args):
+    """One entry of the C ABI on the current stream of `dev`."""
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
-            return _call(name, dev, T, rows, *args)
-    n = capi.call("wd_policy_workspace_floats", rows)
-    if n < 0:
-        raise capi.WdError("wd_policy_workspace_floats failed (%d): %s" % (n, capi.load().wd_last_error().decode()))
-    ws = torch.empty(n, dtype=torch.float32, device=dev)
-    capi.call(name, rows, *args, ws.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+            return _call(name, dev, *args)
+    capi.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))      # the handle current_stream() wraps, without the wrapper's 1 us
 
 
 def sequence_logp(logits, targets, seq_offs, length_norm=False):
     """Log-probabilities of the chosen items: token_logp[r] = log softmax(logits[r])[targets[r]] (0 where the position is no action) and
     seq_logp[n], their sum over sequence n (length_norm: their mean over its actions; 0 without any)."""
-    rows, T, V, N, dev = _rows(logits, targets, seq_offs)
-    out = torch.empty(T + N, dtype=torch.float32, device=dev)
-    p = out.data_ptr()
-    _call("wd_seq_logp", dev, T, rows, int(bool(length_norm)), p, p + 4 * T)
-    return SequenceLogp(out[:T], out[T:])
+    rows, T, V, N, dev, code = _rows(logits, targets, seq_offs)
+    ws = _workspace(T, V, N, code)
+    buf = torch.empty(ws + T + N, dtype=torch.float32, device=dev)      # workspace and results in one allocation
+    p = buf.data_ptr() + 4 * ws
+    _call("wd_seq_logp", dev, rows, int(bool(length_norm)), p, p + 4 * T, buf.data_ptr())
+    _, token, seq = torch.split_with_sizes(buf, (ws, T, N))
+    return SequenceLogp(token, seq)
 
 
 def preference_loss(logits, targets, seq_offs, ref_logp=None, weights=None, beta=0.1, kind="logistic", margin=0.0, label_smoothing=0.0,
@@ -105,7 +115,7 @@ def preference_loss(logits, targets, seq_offs, ref_logp=None, weights=None, beta
     margin; "square": (d - 1 / (2 beta))^2.  loss = sum or mean over the pairs of weights[i] times that.
     dlogits: True (a new tensor), a tensor like logits (rows of no sequence are left as they were; it may be `logits` itself), or None
     (the loss alone); it holds grad_scale times the gradient."""
-    rows, T, V, N, dev = _rows(logits, targets, seq_offs)
+    rows, T, V, N, dev, code = _rows(logits, targets, seq_offs)
     if kind not in PREFERENCE_KINDS or reduction not in ("sum", "mean"):
         raise ValueError("kind is one of %s, reduction sum or mean: got %r, %r" % (sorted(PREFERENCE_KINDS), kind, reduction))
     if N % 2:
@@ -114,12 +124,13 @@ def preference_loss(logits, targets, seq_offs, ref_logp=None, weights=None, beta
     pw = _vector("weights", weights, N // 2, torch.float32, dev) if weights is not None else 0
     g, pg, ldg, tail = _gradient(dlogits, logits)
     P = N // 2
-    out = torch.empty(1 + 2 * P + N + T, dtype=torch.float32, device=dev)
-    p = out.data_ptr()
+    ws = _workspace(T, V, N, code)
+    buf = torch.empty(ws + 1 + 2 * P + N + T, dtype=torch.float32, device=dev)
+    p = buf.data_ptr() + 4 * ws
     opts = _PREF.pack(pr, pw, p, p + 4, p + 4 * (1 + P), p + 4 * (1 + 2 * P), p + 4 * (1 + 2 * P + N), pg, ldg, beta, margin, label_smoothing,
                       1.0 / max(P, 1) if reduction == "mean" else 1.0, grad_scale, PREFERENCE_KINDS[kind], int(bool(length_norm)), tail)
-    _call("wd_pref_loss_fwd_bwd", dev, T, rows, opts)
-    loss, pair, diff, seq, tok = out.split((1, P, P, N, T))
+    _call("wd_pref_loss_fwd_bwd", dev, rows, opts, buf.data_ptr())
+    _, loss, pair, diff, seq, tok = torch.split_with_sizes(buf, (ws, 1, P, P, N, T))
     return PreferenceLoss(loss.view(()), pair, diff, seq, tok, g)
 
 
@@ -132,7 +143,7 @@ def policy_loss(logits, targets, seq_offs, old_logp, advantages, ref_logp=None, 
     actions) or "sequence_mean" (mean over the sequences that have an action of their means).  Returns the loss, and reduced the same way
     k and the share of actions whose clipped side was taken.  old_logp and ref_logp are token_logp of sequence_logp, [rows].
     dlogits as in preference_loss.  per_row: whether advantages are [rows] or [sequences]; None: told by their number, which has to tell."""
-    rows, T, V, N, dev = _rows(logits, targets, seq_offs)
+    rows, T, V, N, dev, code = _rows(logits, targets, seq_offs)
     if reduction not in POLICY_REDUCTIONS:
         raise ValueError("reduction is one of %s: got %r" % (sorted(POLICY_REDUCTIONS), reduction))
     po = _vector("old_logp", old_logp, T, torch.float32, dev)
@@ -146,8 +157,10 @@ def policy_loss(logits, targets, seq_offs, old_logp, advantages, ref_logp=None, 
     pr = _vector("ref_logp", ref_logp, T, torch.float32, dev) if ref_logp is not None else 0
     low, high = clip
     g, pg, ldg, tail = _gradient(dlogits, logits)
-    out = torch.empty(3 + T, dtype=torch.float32, device=dev)
-    p = out.data_ptr()
+    ws = _workspace(T, V, N, code)
+    buf = torch.empty(ws + 3 + T, dtype=torch.float32, device=dev)
+    p = buf.data_ptr() + 4 * ws
     opts = _POLICY.pack(po, pr, pa, p, p + 12, pg, ldg, low, high, kl_coef, grad_scale, int(bool(per_row)), POLICY_REDUCTIONS[reduction], tail, 0)
-    _call("wd_policy_loss_fwd_bwd", dev, T, rows, opts)
-    return PolicyLoss(out[0], out[1], out[2], out[3:], g)
+    _call("wd_policy_loss_fwd_bwd", dev, rows, opts, buf.data_ptr())
+    _, sums, token = torch.split_with_sizes(buf, (ws, 3, T))
+    return PolicyLoss(*sums.unbind(), token, g)
