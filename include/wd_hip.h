@@ -943,7 +943,7 @@ int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy_t *opts, f
  * that is not finite has s = 255 and reads as NaN.  Values are rounded up with the probability of their fraction, by 16 bits for
  * each moment from a hash of (flat index, step, seed): a second moment whose step is below half a code would otherwise never move. */
 #define WD_ADAMW_BLOCK 64
-#define WD_ADAMW_CHUNK 4096   /* elements of one entry of `chunks` */
+#define WD_ADAMW_CHUNK 2048   /* elements of one entry of `chunks` */
 typedef struct wd_adamw_tensor {
   float *p;
   const void *g;
@@ -954,8 +954,9 @@ typedef struct wd_adamw_tensor {
 } wd_adamw_tensor_t;
 typedef struct wd_adamw_state {   /* device; written by wd_adamw_set_step, advanced by every wd_adamw_step that is not skipped */
   int64_t step;              /* steps done */
-  int32_t skipped, ticket;
-  float corr1, corr2;        /* 1 / (1 - b1^(step + 1)), 1 / sqrt(1 - b2^(step + 1)) */
+  int32_t skipped, pad2_;
+  double pow1, pow2;         /* b1^(step + 1), b2^(step + 1) */
+  float corr1, corr2;        /* 1 / (1 - pow1), 1 / sqrt(1 - pow2) */
   float norm, pad_;          /* G of the last step with clipping */
 } wd_adamw_state_t;
 typedef struct wd_adamw {
@@ -965,6 +966,7 @@ typedef struct wd_adamw {
   void *m, *v;               /* v: r's codes with 8 bits */
   uint8_t *m_scale, *r_scale;
   wd_adamw_state_t *state;
+  int32_t *tickets;          /* [WD_ADAMW_TICKETS], zeroed by wd_adamw_set_step, zero between steps */
   double *partials;          /* [WD_ADAMW_PARTIALS], clipping only */
   const float *lr_dev;       /* device [1]: overrides lr (a captured step whose rate moves) */
   double beta1, beta2;
@@ -972,9 +974,10 @@ typedef struct wd_adamw {
   uint32_t seed;
   int32_t bits, grad_dtype, copy_dtype, pad_;
 } wd_adamw_t;
-#define WD_ADAMW_PARTIALS 1024
+#define WD_ADAMW_PARTIALS 2048
+#define WD_ADAMW_TICKETS 1056
 int wd_adamw_step(const wd_adamw_t *opts, wd_stream_t stream);
-int wd_adamw_set_step(wd_adamw_state_t *state, int64_t step, double beta1, double beta2, wd_stream_t stream);
+int wd_adamw_set_step(wd_adamw_state_t *state, int32_t *tickets, int64_t step, double beta1, double beta2, wd_stream_t stream);
 /* 8-bit moments <-> numbers, n values (a multiple of WD_ADAMW_BLOCK) from the start of the flat buffers; unpack: m and r as bf16 or
  * fp32 (bf16 holds every value exactly), pack: to nearest from fp32 m and r. */
 int wd_adamw_unpack(const uint8_t *m, const uint8_t *m_scale, const uint8_t *r, const uint8_t *r_scale, int64_t n, void *out_m,

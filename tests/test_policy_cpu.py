@@ -36,9 +36,11 @@ def test_packed_records_match_the_header(name, fmt):
 
 def test_tensor_and_state_records_match_the_header():
     assert [(n, optim._TENSOR.fields[n][0].itemsize) for n in optim._TENSOR.names][:6] == _struct("wd_adamw_tensor_t")[:6]
-    assert sum(b for _, b in _struct("wd_adamw_state_t")) == 32
+    state = _struct("wd_adamw_state_t")
+    at = {n: sum(b for _, b in state[:k]) // 4 for k, (n, _) in enumerate(state)}
+    assert sum(b for _, b in state) == 48 and (at["step"], at["skipped"], at["norm"]) == (0, 2, 10)       # what optim.py reads
     src = open(os.path.join(ROOT, "include", "wd_hip.h")).read()
-    for name, value in (("BLOCK", optim.BLOCK), ("CHUNK", optim.CHUNK), ("PARTIALS", optim.PARTIALS)):
+    for name, value in (("BLOCK", optim.BLOCK), ("CHUNK", optim.CHUNK), ("PARTIALS", optim.PARTIALS), ("TICKETS", optim.TICKETS)):
         assert int(re.search(r"#define WD_ADAMW_%s (\d+)" % name, src).group(1)) == value
 
 
@@ -82,11 +84,11 @@ def test_policy_options_are_checked(kw, message):
         capi.call("wd_policy_loss_fwd_bwd", _rows(), _policy(**kw), 64, None)
 
 
-def _adamw(tensors=64, chunks=64, n=1, m=64, v=64, ms=64, rs=64, state=64, partials=64, b1=0.9, b2=0.999, eps=1e-8, norm=0.0, bits=32, gt=0, ct=2):
-    return optim._OPTS.pack(tensors, chunks, n, m, v, ms, rs, state, partials, 0, b1, b2, 1e-3, eps, norm, 0, bits, gt, ct, 0)
+def _adamw(tensors=64, chunks=64, n=1, m=64, v=64, ms=64, rs=64, state=64, tickets=64, partials=64, b1=0.9, b2=0.999, eps=1e-8, norm=0.0, bits=32, gt=0, ct=2):
+    return optim._OPTS.pack(tensors, chunks, n, m, v, ms, rs, state, tickets, partials, 0, b1, b2, 1e-3, eps, norm, 0, bits, gt, ct, 0)
 
 
-@pytest.mark.parametrize("kw,message", [(dict(tensors=0), "null pointer"), (dict(n=0), "no chunks"), (dict(state=0), "null pointer"), (dict(bits=16), "32 or in 8"),
+@pytest.mark.parametrize("kw,message", [(dict(tensors=0), "null pointer"), (dict(n=0), "no chunks"), (dict(state=0), "null pointer"), (dict(tickets=0), "null pointer"), (dict(bits=16), "32 or in 8"),
                                         (dict(bits=8, ms=0), "scales"), (dict(gt=3), "gradient type"), (dict(ct=0), "copy"), (dict(b1=1.0), "betas"),
                                         (dict(b2=float("nan")), "betas"), (dict(eps=-1.0), "betas"), (dict(norm=1.0, partials=0), "partials")])
 def test_adamw_options_are_checked(kw, message):
@@ -95,7 +97,7 @@ def test_adamw_options_are_checked(kw, message):
 
 
 def test_adamw_helpers_are_checked():
-    for args in ((None, 0, 0.9, 0.999), (64, -1, 0.9, 0.999), (64, 0, 1.0, 0.999)):
+    for args in ((None, 64, 0, 0.9, 0.999), (64, None, 0, 0.9, 0.999), (64, 64, -1, 0.9, 0.999), (64, 64, 0, 1.0, 0.999)):
         with pytest.raises(capi.WdError, match="wd_adamw_set_step failed"):
             capi.call("wd_adamw_set_step", *args, None)
     with pytest.raises(capi.WdError, match="multiple of the block"):

@@ -265,7 +265,7 @@ _PROTOS = {
     "wd_pref_loss_fwd_bwd": [P, P, P, P],
     "wd_policy_loss_fwd_bwd": [P, P, P, P],
     "wd_adamw_step": [P, P],
-    "wd_adamw_set_step": [P, I64, ctypes.c_double, ctypes.c_double, P],
+    "wd_adamw_set_step": [P, P, I64, ctypes.c_double, ctypes.c_double, P],
     "wd_adamw_unpack": [P, P, P, P, I64, P, P, I32, P],
     "wd_adamw_pack": [P, P, I64, P, P, P, P, P],
     "wd_fill_f32": [P, F32, I64, P],

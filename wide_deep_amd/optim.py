@@ -13,10 +13,10 @@ import torch
 
 from . import capi
 
-BLOCK, CHUNK, PARTIALS = 64, 4096, 1024            # WD_ADAMW_*
+BLOCK, CHUNK, PARTIALS, TICKETS = 64, 2048, 2048, 1056           # WD_ADAMW_*
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _TENSOR = np.dtype([("p", "<u8"), ("g", "<u8"), ("copy", "<u8"), ("n", "<i8"), ("start", "<i8"), ("decay", "<f4"), ("pad", "<i4")])
-_OPTS = struct.Struct("=QQqQQQQQQQddfffIiiii")     # wd_adamw_t
+_OPTS = struct.Struct("=QQqQQQQQQQQddfffIiiii")     # wd_adamw_t
 
 
 class AdamW:
@@ -87,13 +87,14 @@ class AdamW:
             self.m, self.r = torch.zeros(n, **u8), torch.zeros(n, **u8)
             self.m_scale, self.r_scale = torch.full((n // BLOCK,), 27, **u8), torch.full((n // BLOCK,), 27, **u8)
             second, scales = self.r, (self.m_scale.data_ptr(), self.r_scale.data_ptr())
-        self._state = torch.zeros(8, dtype=torch.int32, device=dev)      # wd_adamw_state_t
+        self._state = torch.zeros(12, dtype=torch.int32, device=dev)      # wd_adamw_state_t
+        self._tickets = torch.empty(TICKETS, dtype=torch.int32, device=dev)
         #: global norm of the gradients of the last step with max_norm, before clipping; the next step writes it
-        self.grad_norm = self._state[6:7].view(torch.float32)[0]
+        self.grad_norm = self._state[10:11].view(torch.float32)[0]
         self._partials = torch.zeros(PARTIALS, dtype=torch.float64, device=dev) if max_norm is not None else None
         self._device = dev
         self._head = (self._tensors.data_ptr(), self._chunks.data_ptr(), len(chunks), self.m.data_ptr(), second.data_ptr(), *scales,
-                      self._state.data_ptr(), 0 if self._partials is None else self._partials.data_ptr())
+                      self._state.data_ptr(), self._tickets.data_ptr(), 0 if self._partials is None else self._partials.data_ptr())
         self._tail = (*self.betas,)
         self._types = (state_bits, _DTYPES[grads[0].dtype], _DTYPES[copy_type.pop()] if copy_type else 2, 0)
         self.set_step(0)
@@ -116,7 +117,7 @@ class AdamW:
 
     def set_step(self, step):
         """The number of steps done so far (a restored optimizer); clears `skipped`."""
-        self._call("wd_adamw_set_step", self._state.data_ptr(), int(step), *self.betas)
+        self._call("wd_adamw_set_step", self._state.data_ptr(), self._tickets.data_ptr(), int(step), *self.betas)
 
     @property
     def step_count(self):
