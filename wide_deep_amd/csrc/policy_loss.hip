@@ -103,7 +103,10 @@ template <int DT> struct Row {
     nb = (V - head) / W;
     rest = V - head - nb * W;
   }
-  __device__ __forceinline__ u32x4 word(int j) const { return *(const u32x4 *)(p + head + j * W); }
+  template <bool NT = false> __device__ __forceinline__ u32x4 word(int j) const {
+    const u32x4 *q = (const u32x4 *)(p + head + j * W);
+    return NT ? __builtin_nontemporal_load(q) : *q;
+  }
   // the element outside the words that lane i takes, -1: none
   __device__ __forceinline__ int edge(int i) const { return i < head ? i : i < head + rest ? i + nb * W : -1; }
 };
@@ -118,8 +121,8 @@ template <int N> __device__ __forceinline__ void hold(u32x4 (&w)[N]) {
   for (int u = 0; u < N; ++u) asm volatile("" : "+v"(w[u]));
 }
 template <int DT> __device__ __forceinline__ void store_word(typename Elem<DT>::type *g, bool aligned, const float *x) {
-  if (aligned) {
-    *(u32x4 *)g = Elem<DT>::pack(x);
+  if (aligned) {      // the gradient is not read here: it need not push the logits out of the last cache (policy, odd catalogue: 48 -> 36 us)
+    __builtin_nontemporal_store(Elem<DT>::pack(x), (u32x4 *)g);
     return;
   }
 #pragma unroll
@@ -189,7 +192,8 @@ __device__ __forceinline__ bool is_action(const wd_seq_rows_t &q, int32_t t) { r
 __device__ __forceinline__ float logp(float xt, float m, float s) { return (xt - m) - logf(s); }
 
 // ---- (m, s) of every part of every row: workgroup (row, part).  A row in one part is done here, its log-probability too.
-template <int DT>
+// NT: logits that the last cache cannot keep for a later pass anyway are read past it (0.39 GB: 87 -> 82 us)
+template <int DT, bool NT>
 __global__ void __launch_bounds__(256)
 k_row_stats(wd_seq_rows_t q, int32_t nsplit, float2 *__restrict__ part, float2 *__restrict__ stat, float *__restrict__ token) {
   constexpr int TH = 256, U = 4, W = Elem<DT>::W;
@@ -219,7 +223,7 @@ k_row_stats(wd_seq_rows_t q, int32_t nsplit, float2 *__restrict__ part, float2 *
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       w[u] = no_word<DT>();
-      if (j + u * TH < j1) w[u] = row.word(j + u * TH);
+      if (j + u * TH < j1) w[u] = row.template word<NT>(j + u * TH);
     }
     hold(w);
     float x[U * W], M = m;
@@ -388,52 +392,60 @@ template <int TH> __device__ __forceinline__ void weighted_sum(const float *v, c
   if (threadIdx.x == 0) *out = (float)(t * scale);
 }
 
-// part z of a row's gradient; c = 0 for a row that is no action (m = 0, s = 1; its logits are not read)
-template <int DT, int TH>
-__device__ __forceinline__ void grad_part(const Row<DT> &row, typename Elem<DT>::type *g, int z, int nsplit, bool action, int32_t t, float m,
-                                          float s, float c) {
+struct RowScalars {
+  float m, s, c;
+};
+// part z of a row's gradient; zeros for a row that is no action (its logits are not read).  scalars() is asked for (m, s, c) when the first
+// words are on their way.
+template <int DT, int TH, bool NT, typename F>
+__device__ __forceinline__ void grad_part(const Row<DT> &row, typename Elem<DT>::type *g, int z, int nsplit, bool action, int32_t t, F scalars) {
   constexpr int W = Elem<DT>::W, U = 4;
   const int per = (row.nb + nsplit - 1) / nsplit;
-  const int j1 = min(row.nb, (z + 1) * per), jt = t < row.head ? -1 : (t - row.head) / W;
+  const int j0 = z * per, j1 = min(row.nb, (z + 1) * per), jt = t < row.head ? -1 : (t - row.head) / W;
   typename Elem<DT>::type *gb = g + row.head;
   const bool aligned = ((uintptr_t)gb & 15) == 0;
-  const float k = -c / s;
-  if (z == 0) {
-    const int e = row.edge(threadIdx.x);
-    if (e >= 0) g[e] = Elem<DT>::from_float(action ? k * exp_rel(Elem<DT>::to_float(row.p[e]), m) + (e == t ? c : 0.f) : 0.f);
-  }
+  const int e = z == 0 ? row.edge(threadIdx.x) : -1;
   float x[W];
-  for (int j = z * per + threadIdx.x; j < j1; j += TH * U) {
+  if (!action) {
+    if (e >= 0) g[e] = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) x[i] = 0.f;
+    for (int j = j0 + threadIdx.x; j < j1; j += TH) store_word<DT>(gb + j * W, aligned, x);
+    return;
+  }
+  RowScalars k;
+  for (int jw = j0; jw < j1 || jw == j0; jw += TH * U) {      // once at least: a short row may be all edge
+    const int j = jw + threadIdx.x;
     u32x4 w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-    {
+    for (int u = 0; u < U; ++u) {
       w[u] = no_word<DT>();
-      if (action && j + u * TH < j1) w[u] = row.word(j + u * TH);
+      if (j + u * TH < j1) w[u] = row.template word<NT>(j + u * TH);
+    }
+    if (jw == j0) {
+      const float xe = e >= 0 ? Elem<DT>::to_float(row.p[e]) : 0.f;
+      k = scalars();
+      k.s = -k.c / k.s;
+      if (e >= 0) g[e] = Elem<DT>::from_float(k.s * exp_rel(xe, k.m) + (e == t ? k.c : 0.f));
     }
     hold(w);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int ju = j + u * TH;
       if (ju >= j1) break;
-      if (action) {
-        Elem<DT>::unpack(w[u], x);
+      Elem<DT>::unpack(w[u], x);
 #pragma unroll
-        for (int i = 0; i < W; ++i) x[i] = k * exp_rel(x[i], m);
-        if (ju == jt) {
+      for (int i = 0; i < W; ++i) x[i] = k.s * exp_rel(x[i], k.m);
+      if (ju == jt) {
 #pragma unroll
-          for (int i = 0; i < W; ++i) x[i] += row.head + ju * W + i == t ? c : 0.f;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < W; ++i) x[i] = 0.f;
+        for (int i = 0; i < W; ++i) x[i] += row.head + ju * W + i == t ? k.c : 0.f;
       }
       store_word<DT>(gb + ju * W, aligned, x);
     }
   }
 }
 
-template <int DT>
+template <int DT, bool NT>
 __global__ void __launch_bounds__(256)
 k_logits_grad(wd_seq_rows_t q, void *dlogits, int64_t ldg, int32_t zero_tail, int32_t nsplit, const float2 *__restrict__ stat,
               const float *__restrict__ coef, const float *__restrict__ pair_loss, const float *__restrict__ weights, double scale,
@@ -449,8 +461,10 @@ k_logits_grad(wd_seq_rows_t q, void *dlogits, int64_t ldg, int32_t zero_tail, in
   const int32_t t = q.targets[r];
   const bool action = !tail && is_action(q, t);
   const Row<DT> row(q.logits, q.ld, r, (int)q.vocab);
-  const float2 ms = action ? stat[r] : make_float2(0.f, 1.f);
-  grad_part<DT, TH>(row, (typename Elem<DT>::type *)dlogits + r * ldg, z, nsplit, action, t, ms.x, ms.y, action ? coef[r] : 0.f);
+  grad_part<DT, TH, NT>(row, (typename Elem<DT>::type *)dlogits + r * ldg, z, nsplit, action, t, [&] {
+    const float2 ms = stat[r];
+    return RowScalars{ms.x, ms.y, coef[r]};
+  });
 }
 
 // sequence of row r, by a wavefront: the number of sequences that end in front of it
@@ -506,16 +520,13 @@ __global__ void __launch_bounds__(256) k_pref_grad(wd_seq_rows_t q, wd_pref_t o,
   const int32_t t = q.targets[r];
   const bool action = !tail && is_action(q, t);
   const Row<DT> row(q.logits, q.ld, r, (int)q.vocab);
-  float2 ms = make_float2(0.f, 1.f);
-  float c = 0.f;
-  if (action) {
-    ms = stat[r];
+  grad_part<DT, TH, false>(row, (typename Elem<DT>::type *)o.dlogits + r * o.ld_dlogits, z, nsplit, action, t, [&] {
+    const float2 ms = stat[r];
     const int64_t s = wave_sequence(q, r);
     wave_pair(q, o, s / 2, lp, n);
     const double slope = pair_slope(o, s / 2, pair_difference(o, s / 2, lp[0], lp[1]));
-    c = (float)(s & 1 ? -slope / n[1] : slope / n[0]);
-  }
-  grad_part<DT, TH>(row, (typename Elem<DT>::type *)o.dlogits + r * o.ld_dlogits, z, nsplit, action, t, ms.x, ms.y, c);
+    return RowScalars{ms.x, ms.y, (float)(s & 1 ? -slope / n[1] : slope / n[0])};
+  });
 }
 
 // ---- clipped policy loss
@@ -606,7 +617,7 @@ k_policy_resident(wd_seq_rows_t q, wd_policy_t o, const float *__restrict__ w, c
       o.token_logp[r] = 0.f;
       rows3[r] = rows3[q.rows + r] = rows3[2 * q.rows + r] = 0.f;
     }
-    if (o.dlogits) grad_part<DT, TH>(row, g, 0, 1, false, -1, 0.f, 1.f, 0.f);
+    if (o.dlogits) grad_part<DT, TH, false>(row, g, 0, 1, false, -1, [] { return RowScalars{0.f, 1.f, 0.f}; });
     return;
   }
   u32x4 v[NV];
@@ -736,7 +747,7 @@ int row_split(const wd_seq_rows_t &q) {
 int grad_split(const wd_seq_rows_t &q) { return words(q) <= 1024 ? 1 : (int)ceil_div(words(q), 1024); }
 
 // batches whose rows find their pair, weight or advantage themselves instead of in a launch of its own
-constexpr int64_t kSelfRows = 256, kSelfSeqs = 256;
+constexpr int64_t kSelfRows = 256, kSelfSeqs = 256, kPairRows = 2048;
 // whole words of the longest row that a workgroup holds in registers: 1024 lanes x 16
 constexpr int kResidentWords = 16384;
 
@@ -767,9 +778,29 @@ template <typename F> void by_type(int32_t dtype, F f) {
   else f(std::integral_constant<int, WD_T_BF16>());
 }
 
-void launch_stats(const wd_seq_rows_t &q, int nsplit, const Work &k, float *token, hipStream_t st) {
+// more logits than the last cache (256 MB) holds
+bool beyond_cache(const wd_seq_rows_t &q) { return q.rows * q.ld * (q.dtype == WD_T_F32 ? 4 : 2) > ((int64_t)256 << 20); }
+
+// `again`: another pass reads the logits afterwards
+void launch_stats(const wd_seq_rows_t &q, int nsplit, const Work &k, float *token, bool again, hipStream_t st) {
   if (q.rows < 1) return;
-  by_type(q.dtype, [&](auto dt) { k_row_stats<decltype(dt)::value><<<row_grid(q.rows, nsplit), 256, 0, st>>>(q, nsplit, k.part, k.stat, token); });
+  by_type(q.dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    const dim3 grid = row_grid(q.rows, nsplit);
+    if (!again && beyond_cache(q)) k_row_stats<DT, true><<<grid, 256, 0, st>>>(q, nsplit, k.part, k.stat, token);
+    else k_row_stats<DT, false><<<grid, 256, 0, st>>>(q, nsplit, k.part, k.stat, token);
+  });
+}
+// the gradient is the last to read the logits: 1.14 GB 489 -> 448 us past the cache, 61 MB 33 -> 36 us
+template <int DT>
+void launch_grad(const wd_seq_rows_t &q, int64_t rows, void *dlogits, int64_t ldg, int32_t zero_tail, const Work &k, const float *pair_loss,
+                 const float *weights, double scale, float *loss, hipStream_t st) {
+  wd_seq_rows_t last = q;
+  last.rows = rows;
+  const int gs = grad_split(q);
+  const dim3 grid = row_grid(rows + (loss ? 1 : 0), gs);
+  if (beyond_cache(q)) k_logits_grad<DT, true><<<grid, 256, 0, st>>>(last, dlogits, ldg, zero_tail, gs, k.stat, k.coef, pair_loss, weights, scale, loss);
+  else k_logits_grad<DT, false><<<grid, 256, 0, st>>>(last, dlogits, ldg, zero_tail, gs, k.stat, k.coef, pair_loss, weights, scale, loss);
 }
 
 // A row in the registers of a workgroup, NV words a lane.  Two or more workgroups have to fit on a CU, so that one loads or stores while
@@ -812,7 +843,7 @@ extern "C" int wd_seq_logp(const wd_seq_rows_t *rows, int32_t length_norm, float
   hipStream_t st = as_stream(stream);
   const Work k(q, ws);
   const int ns = row_split(q);
-  launch_stats(q, ns, k, token_logp, st);
+  launch_stats(q, ns, k, token_logp, false, st);
   if (q.nseq > 0) by_type(q.dtype, [&](auto dt) {
     k_seq_logp<decltype(dt)::value><<<row_grid(q.nseq, 1), 256, 0, st>>>(q, ns, length_norm, k.part, k.stat, token_logp, seq_logp);
   });
@@ -834,19 +865,17 @@ extern "C" int wd_pref_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_pref_t *
   WD_REQUIRE((uintptr_t)o.dlogits % (q.dtype == WD_T_F32 ? 4 : 2) == 0, "gradient not aligned to its element size");
   hipStream_t st = as_stream(stream);
   const Work k(q, ws);
-  const int ns = row_split(q), gs = grad_split(q);
-  launch_stats(q, ns, k, o.token_logp, st);
-  wd_seq_rows_t last = q;
-  if (!o.dlogits) last.rows = 0;      // the loss alone
+  const int ns = row_split(q);
+  launch_stats(q, ns, k, o.token_logp, o.dlogits != nullptr, st);
   by_type(q.dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (ns == 1 && q.rows <= kSelfRows && q.nseq <= kSelfSeqs) {
+    if (ns == 1 && q.rows <= kPairRows && q.nseq <= kSelfSeqs) {
+      const int gs = (int)ceil_div(grad_split(q), 4);
       k_pref_grad<DT><<<row_grid(q.rows + 1, gs), 256, 0, st>>>(q, o, gs, k.stat);
       return;
     }
     if (q.nseq > 0) k_pref_pairs<DT><<<row_grid(q.nseq / 2, 1), 256, 0, st>>>(q, o, ns, k.part, k.stat, k.coef);
-    k_logits_grad<DT><<<row_grid(last.rows + 1, gs), 256, 0, st>>>(last, o.dlogits, o.ld_dlogits, o.zero_tail, gs, k.stat, k.coef, o.pair_loss,
-                                                                   o.weights, (double)o.scale, o.loss);
+    launch_grad<DT>(q, o.dlogits ? q.rows : 0, o.dlogits, o.ld_dlogits, o.zero_tail, k, o.pair_loss, o.weights, (double)o.scale, o.loss, st);
   });
   return check_launch(__func__);
 }
@@ -875,12 +904,10 @@ extern "C" int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy
     by_type(q.dtype, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
       if (!launch_resident<DT>(q, o, k, st)) {
-        const int ns = row_split(q), gs = grad_split(q);
-        launch_stats(q, ns, k, o.token_logp, st);
+        const int ns = row_split(q);
+        launch_stats(q, ns, k, o.token_logp, o.dlogits != nullptr, st);
         k_policy_join<DT><<<dim3((unsigned)ceil_div(q.rows * ns, 256)), 256, 0, st>>>(q, o, ns, k.part, k.w, k.adv, k.cnt, k.stat, k.coef, k.rows3);
-        if (o.dlogits)
-          k_logits_grad<DT><<<row_grid(q.rows, gs), 256, 0, st>>>(q, o.dlogits, o.ld_dlogits, o.zero_tail, gs, k.stat, k.coef, nullptr,
-                                                                           nullptr, 0.0, nullptr);
+        if (o.dlogits) launch_grad<DT>(q, q.rows, o.dlogits, o.ld_dlogits, o.zero_tail, k, nullptr, nullptr, 0.0, nullptr, st);
       }
     });
   }
