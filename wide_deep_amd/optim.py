@@ -100,7 +100,7 @@ class AdamW:
         self.set_step(0)
 
     def _call(self, name, *args):
-        if torch.cuda.current_device() != self._device.index:
+        if torch._C._cuda_getDevice() != self._device.index:
             with torch.cuda.device(self._device):
                 return self._call(name, *args)
         return capi.call(name, *args, torch._C._cuda_getCurrentRawStream(self._device.index))

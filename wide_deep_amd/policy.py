@@ -41,24 +41,30 @@ def _what(t):
     return "%s %s on %s" % (t.dtype, list(t.shape), t.device) if isinstance(t, torch.Tensor) else repr(t)
 
 
+def _layout(name, t, V):
+    """Row stride of a [rows, V] tensor."""
+    if t.is_contiguous() and V > 0:
+        return V
+    step, item = t.stride()
+    T = t.shape[0]
+    if V < 1 or (T and V > 1 and item != 1) or (T > 1 and step < V):
+        raise ValueError("%s: at least one item, items contiguous, rows not overlapping are wanted, got %s with strides %s" % (name, _what(t), t.stride()))
+    return step if T > 1 else V
+
+
 def _rows(logits, targets, seq_offs):
     """wd_seq_rows_t of a batch, packed, after the checks that need no device."""
-    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _DTYPES:
+    code = _DTYPES.get(logits.dtype) if isinstance(logits, torch.Tensor) and logits.dim() == 2 else None
+    if code is None:
         raise ValueError("logits: a [rows, vocab] tensor of fp32, fp16 or bf16 is wanted, got %s" % _what(logits))
     T, V = logits.shape
-    ld = V
-    if not logits.is_contiguous() or V < 1:
-        step, item = logits.stride()
-        if V < 1 or (T and V > 1 and item != 1) or (T > 1 and step < V):
-            raise ValueError("logits: at least one item, items contiguous, rows not overlapping are wanted, got %s with strides %s" % (_what(logits), logits.stride()))
-        ld = step if T > 1 else V
+    ld = _layout("logits", logits, V)
     dev = logits.device
     if dev.type != "cuda":
         raise capi.WdError("policy heads need a GPU (MI355X / gfx950); there is no CPU fallback: logits are on %s" % dev)
     pt = _vector("targets", targets, T, torch.int32, dev)
     N = seq_offs.numel() - 1 if isinstance(seq_offs, torch.Tensor) else 0
     po = _vector("seq_offs", seq_offs, max(N, 0) + 1, torch.int32, dev)
-    code = _DTYPES[logits.dtype]
     return _ROWS.pack(logits.data_ptr(), ld, T, V, pt, po, N, code, 0), T, V, N, dev, code
 
 
@@ -78,20 +84,23 @@ def _gradient(dlogits, logits):
         return g, g.data_ptr(), logits.shape[1], 1       # rows of no sequence: zeros
     if dlogits is None or dlogits is False:
         return None, 0, 0, 0
-    if not isinstance(dlogits, torch.Tensor) or dlogits.shape != logits.shape or dlogits.dtype != logits.dtype or dlogits.device != logits.device:
+    if not isinstance(dlogits, torch.Tensor) or dlogits.shape != logits.shape or dlogits.dtype is not logits.dtype or dlogits.device != logits.device:
         raise ValueError("dlogits: a tensor like logits (%s) is wanted, got %s" % (_what(logits), _what(dlogits)))
-    T, V = dlogits.shape
-    if (T and V > 1 and dlogits.stride(1) != 1) or (T > 1 and dlogits.stride(0) < V):
-        raise ValueError("dlogits: items contiguous, rows not overlapping are wanted, got strides %s" % (dlogits.stride(),))
-    return dlogits, dlogits.data_ptr(), dlogits.stride(0) if T > 1 else V, 0
+    return dlogits, dlogits.data_ptr(), _layout("dlogits", dlogits, logits.shape[1]), 0
 
 
 def _call(name, dev, *args):
     """One entry of the C ABI on the current stream of `dev`."""
-    if torch.cuda.current_device() != dev.index:
+    if torch._C._cuda_getDevice() != dev.index:
         with torch.cuda.device(dev):
             return _call(name, dev, *args)
     capi.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))      # the handle current_stream() wraps, without the wrapper's 1 us
+
+
+def _buffer(logits, *sizes):
+    """Workspace and results of a call in one allocation: its address and its parts."""
+    buf = logits.new_empty(sum(sizes), dtype=torch.float32)
+    return buf.data_ptr(), torch.unsafe_split_with_sizes(buf, sizes)
 
 
 def sequence_logp(logits, targets, seq_offs, length_norm=False):
@@ -99,10 +108,9 @@ def sequence_logp(logits, targets, seq_offs, length_norm=False):
     seq_logp[n], their sum over sequence n (length_norm: their mean over its actions; 0 without any)."""
     rows, T, V, N, dev, code = _rows(logits, targets, seq_offs)
     ws = _workspace(T, V, N, code)
-    buf = torch.empty(ws + T + N, dtype=torch.float32, device=dev)      # workspace and results in one allocation
-    p = buf.data_ptr() + 4 * ws
-    _call("wd_seq_logp", dev, rows, int(bool(length_norm)), p, p + 4 * T, buf.data_ptr())
-    _, token, seq = torch.split_with_sizes(buf, (ws, T, N))
+    base, (_, token, seq) = _buffer(logits, ws, T, N)
+    p = base + 4 * ws
+    _call("wd_seq_logp", dev, rows, int(bool(length_norm)), p, p + 4 * T, base)
     return SequenceLogp(token, seq)
 
 
@@ -125,13 +133,12 @@ def preference_loss(logits, targets, seq_offs, ref_logp=None, weights=None, beta
     g, pg, ldg, tail = _gradient(dlogits, logits)
     P = N // 2
     ws = _workspace(T, V, N, code)
-    buf = torch.empty(ws + 1 + 2 * P + N + T, dtype=torch.float32, device=dev)
-    p = buf.data_ptr() + 4 * ws
+    base, (_, loss, pair, diff, seq, tok) = _buffer(logits, ws, 1, P, P, N, T)
+    p = base + 4 * ws
     opts = _PREF.pack(pr, pw, p, p + 4, p + 4 * (1 + P), p + 4 * (1 + 2 * P), p + 4 * (1 + 2 * P + N), pg, ldg, beta, margin, label_smoothing,
                       1.0 / max(P, 1) if reduction == "mean" else 1.0, grad_scale, PREFERENCE_KINDS[kind], int(bool(length_norm)), tail)
-    _call("wd_pref_loss_fwd_bwd", dev, rows, opts, buf.data_ptr())
-    _, loss, pair, diff, seq, tok = torch.split_with_sizes(buf, (ws, 1, P, P, N, T))
-    return PreferenceLoss(loss.view(()), pair, diff, seq, tok, g)
+    _call("wd_pref_loss_fwd_bwd", dev, rows, opts, base)
+    return PreferenceLoss(loss.squeeze(), pair, diff, seq, tok, g)
 
 
 def policy_loss(logits, targets, seq_offs, old_logp, advantages, ref_logp=None, per_row=None, clip=(0.2, 0.2), kl_coef=0.0, reduction="token_mean",
@@ -158,9 +165,8 @@ def policy_loss(logits, targets, seq_offs, old_logp, advantages, ref_logp=None, 
     low, high = clip
     g, pg, ldg, tail = _gradient(dlogits, logits)
     ws = _workspace(T, V, N, code)
-    buf = torch.empty(ws + 3 + T, dtype=torch.float32, device=dev)
-    p = buf.data_ptr() + 4 * ws
+    base, (_, sums, token) = _buffer(logits, ws, 3, T)
+    p = base + 4 * ws
     opts = _POLICY.pack(po, pr, pa, p, p + 12, pg, ldg, low, high, kl_coef, grad_scale, int(bool(per_row)), POLICY_REDUCTIONS[reduction], tail, 0)
-    _call("wd_policy_loss_fwd_bwd", dev, rows, opts, buf.data_ptr())
-    _, sums, token = torch.split_with_sizes(buf, (ws, 3, T))
+    _call("wd_policy_loss_fwd_bwd", dev, rows, opts, base)
     return PolicyLoss(*sums.unbind(), token, g)
