@@ -216,6 +216,69 @@ def test_policy_loss(dtype, vocab, reduction, per_row, kl):
     untouched(b, flat, grad, 0, 0)
 
 
+def check_all(b, name=""):
+    """Scores, both preference losses and the policy loss with every reduction against their definitions."""
+    from wide_deep_amd import policy
+    lp, _, _, tol, _ = b.reference()
+    r = policy.sequence_logp(b.z, b.targets, b.offs)
+    check(name + "token", r.token_logp, lp, tol)
+    check(name + "sequence", r.seq_logp, b.sums(lp), b.sums(tol) + 2 * U * b.sums(lp).abs())
+    rows = slice(int(b.offs[0]), int(b.offs[-1]))
+    for kind, norm in (("logistic", False), ("square", True)):
+        n = b.sums(b.live.double()).clamp(min=1) if norm else 1.0
+        ref = (b.sums(lp) / n + b.rand(b.N, 2.0)).float()
+        w = torch.rand(b.N // 2, device="cuda", generator=b.g) + 0.5
+        want = pair_reference(b, ref, w, 0.1, kind, 0.0, 0.0, norm, 1.0, 16.0)
+        r = policy.preference_loss(b.z, b.targets, b.offs, ref_logp=ref, weights=w, beta=0.1, kind=kind, length_norm=norm, grad_scale=16.0)
+        for key, got in (("token", r.token_logp), ("seq", r.seq_logp), ("diff", r.difference), ("pair", r.pair_loss), ("loss", r.loss)):
+            v, t = want[key]
+            # beta, margin and scale reach the kernel as fp32: 2^-24 relative of each
+            slack = 16 * U * (v.abs() + (want["diff"][0].abs().max() + 5) * (1.0 if key == "pair" else b.N if key == "loss" else 0.0))
+            check("%s%s %s" % (name, kind, key), got, v, t + slack)
+        v, t = want["grad"]
+        check("%s%s gradient" % (name, kind), r.dlogits[rows], v[rows], t[rows] + 16 * U * v[rows].abs().amax())
+        assert bool((r.dlogits[rows.stop:] == 0).all()) and bool((r.dlogits[:rows.start] == 0).all())
+    for reduction, per_row, kl in (("sum", False, 0.1), ("token_mean", True, 0.0), ("sequence_mean", False, 0.1)):
+        check_policy(b, reduction, per_row, kl, name)
+
+
+def check_policy(b, reduction, per_row, kl, name=""):
+    from wide_deep_amd import policy
+    lp = b.reference()[0]
+    shift = b.rand(b.T, 0.2).double()
+    for edge in (math.log1p(0.3), math.log1p(-0.2)):
+        shift = torch.where((shift - edge).abs() < 1e-3, shift + 3e-3, shift)
+    old, ref = (lp - shift).float(), (lp + b.rand(b.T, 0.3)).float() if kl else None
+    adv = b.rand(b.T if per_row else b.N)
+    want = policy_reference(b, old, adv if per_row else b.by_row(adv), ref, (0.2, 0.3), kl, reduction, 32.0)
+    r = policy.policy_loss(b.z, b.targets, b.offs, old, adv, ref_logp=ref, per_row=per_row, clip=(0.2, 0.3), kl_coef=kl, reduction=reduction, grad_scale=32.0)
+    for key, got in (("token", r.token_logp), ("loss", r.loss), ("kl", r.kl), ("clipped", r.clipped)):
+        check("%s%s %s" % (name, reduction, key), got, *want[key])
+    rows = slice(int(b.offs[0]), int(b.offs[-1]))
+    check("%s%s gradient" % (name, reduction), r.dlogits[rows], want["grad"][0][rows], want["grad"][1][rows])
+    assert bool((r.dlogits[rows.stop:] == 0).all())
+
+
+@pytest.mark.parametrize("rows,seqs,vocab,dtype", [(70, 6, 2048, "f32"), (70, 6, 4096, "bf16"), (66, 64, 900, "f16"), (300, 10, 8193, "f32"), (300, 30, 33001, "bf16"),
+                                                   (257, 258, 700, "bf16"), (2100, 12, 301, "f16"), (2100, 40, 9001, "bf16"), (5000, 1600, 37, "f32"), (70000, 1200, 5, "f16")])
+def test_ways_of_the_kernels(rows, seqs, vocab, dtype):
+    """Batches on either side of the limits at which the launches change: rows and sequences that are many or few, rows short or split."""
+    g = torch.Generator().manual_seed(rows + seqs)
+    seqs += seqs % 2
+    share = torch.rand(seqs, generator=g) * (torch.rand(seqs, generator=g) < 0.9)
+    lengths = (share / share.sum() * rows).floor().int().tolist()
+    masked = [n if k % 7 == 3 else n // 4 for k, n in enumerate(lengths)]
+    check_all(Batch(lengths, masked, vocab, DTYPES[dtype], seed=rows, front=1, spare=rows - sum(lengths) - 1))
+
+
+@pytest.mark.parametrize("words", [1, 65, 128, 129, 257, 400, 513, 1100, 2048, 2049, 3100, 4097, 4700, 5200, 5700, 6200, 6700, 7200, 8200, 9300, 10300, 11300, 12800,
+                                   12801, 14400, 16384, 16385])
+def test_policy_rows_of_every_register_count(words):
+    """One row length for each number of 16-byte words a lane may hold, and its neighbours at the limits."""
+    check_policy(Batch([3, 2], [1, 0], 8 * words + 3, torch.bfloat16, seed=words), "sequence_mean", False, 0.1)
+    check_policy(Batch([2, 200, 100], [1, 0, 50], 8 * words - 1, torch.bfloat16, seed=words), "token_mean", True, 0.0)
+
+
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("pad,shift,gpad,gshift", [(0, 1, 0, 1), (3, 0, 3, 0), (5, 3, 0, 0), (0, 0, 1, 2), (8, 0, 8, 4)])
 def test_strides_and_alignments(dtype, pad, shift, gpad, gshift):
@@ -393,6 +456,21 @@ def test_streams_graphs_and_shared_buffers():
     assert same(r, want[:6]) and r.dlogits is z
     z = b.z.clone()
     assert same(policy.policy_loss(z, b.targets, b.offs, old[id(b)], adv, dlogits=z), want[6:11])
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(400, 9001, "bf16"), (90, 60001, "f32"), (9, 300001, "bf16"), (600, 20001, "f16"), (3000, 501, "f32"), (40, 200, "f32")])
+def test_gradient_in_the_place_of_the_logits(rows, vocab, dtype):
+    """The same bits whether the gradient has a buffer of its own or the logits': no launch reads a logit that another row's may overwrite."""
+    from wide_deep_amd import policy
+    n = rows // 4
+    b = Batch([n, n, n, rows - 3 * n], [1, 0, n // 2, 0], vocab, DTYPES[dtype], seed=rows)
+    old, adv = b.reference()[0].float() - 0.1, b.rand(4)
+    for call in (lambda z, g: policy.preference_loss(z, b.targets, b.offs, dlogits=g), lambda z, g: policy.policy_loss(z, b.targets, b.offs, old, adv, per_row=False, dlogits=g)):
+        want = call(b.z, True)
+        for _ in range(8):
+            z = b.z.clone()
+            got = call(z, z)
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
 def test_offsets_past_32_bits():

@@ -124,7 +124,8 @@ def test_python_entry_points_refuse_before_the_device():
                         (dict(grads=[g[0], g[1].half()]), "gradient 1"), (dict(params=[p[0].double(), p[1]]), "parameter 0"),
                         (dict(params=[p[0].t().contiguous().t(), p[1]]), "parameter 0"), (dict(weight_decay=[0.1]), "weight decays"),
                         (dict(betas=(1.0, 0.9)), "betas"), (dict(state_bits=16), "state_bits"), (dict(max_norm=0.0), "max_norm"),
-                        (dict(copies=[p[0].half(), p[1].bfloat16()]), "one half type"), (dict(copies=[None, p[0].half()]), "copy 1")):
+                        (dict(copies=[p[0].half(), p[1].bfloat16()]), "one half type"), (dict(copies=[None, p[0].half()]), "copy 1"), (dict(params=[p[0], p[0][1]], grads=[g[0], g[0][1]]), "share memory"),
+                        (dict(params=[p[0], p[0]], grads=[g[0], g[0]]), "share memory")):
         with pytest.raises(ValueError, match=message):
             optim.AdamW(**{**dict(params=p, grads=g), **kw})
 

@@ -20,6 +20,8 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
+// batches whose rows find their pair, weight or advantage themselves instead of in a launch of its own
+constexpr int64_t kSelfRows = 256, kSelfSeqs = 256, kPairRows = 2048;
 constexpr int64_t kCountSeqs = 1024;      // up to as many sequences every wavefront adds the counts up itself
 constexpr float kLowest = -3.402823466e38f;
 
@@ -191,39 +193,41 @@ __device__ __forceinline__ bool is_action(const wd_seq_rows_t &q, int32_t t) { r
 
 __device__ __forceinline__ float logp(float xt, float m, float s) { return (xt - m) - logf(s); }
 
-// ---- (m, s) of every part of every row: workgroup (row, part).  A row in one part is done here, its log-probability too.
-// NT: logits that the last cache cannot keep for a later pass anyway are read past it (0.39 GB: 87 -> 82 us)
-template <int DT, bool NT>
+// ---- (m, s) of every part of every row: LANES = 256, a workgroup a part; 64, a wavefront a (short) row.  A row in one part is done here,
+// its log-probability too.  NT: logits that the last cache cannot keep for a later pass anyway are read past it (0.39 GB: 87 -> 82 us)
+template <int DT, int LANES, bool NT>
 __global__ void __launch_bounds__(256)
-k_row_stats(wd_seq_rows_t q, int32_t nsplit, float2 *__restrict__ part, float2 *__restrict__ stat, float *__restrict__ token) {
-  constexpr int TH = 256, U = 4, W = Elem<DT>::W;
-  __shared__ float lm[TH / kWave], ls[TH / kWave];
-  const int64_t r = block_row();
-  const int z = (int)blockIdx.x;
+k_row_stats(wd_seq_rows_t q, int32_t nsplit, float2 *__restrict__ part, float *__restrict__ pick, float2 *__restrict__ stat,
+            float *__restrict__ token) {
+  constexpr int U = 4, W = Elem<DT>::W, ROWS = 256 / LANES;
+  __shared__ float lm[256 / kWave], ls[256 / kWave];
+  const int64_t r = block_row() * ROWS + threadIdx.x / LANES;
+  const int z = (int)blockIdx.x, lane = threadIdx.x & (LANES - 1);
   if (r >= q.rows) return;
   const int32_t t = q.targets[r];
   if (outside(q, r) || !is_action(q, t)) {
-    if (z == 0 && threadIdx.x == 0) token[r] = 0.f;
+    if (z == 0 && lane == 0) token[r] = 0.f;
     return;
   }
   const Row<DT> row(q.logits, q.ld, r, (int)q.vocab);
   const int per = (row.nb + nsplit - 1) / nsplit;
   const int j1 = min(row.nb, (z + 1) * per);
+  const float xt = Elem<DT>::to_float(row.p[t]);
   float m = kLowest, s = 0.f;
   if (z == 0) {
-    const int e = row.edge(threadIdx.x);
+    const int e = row.edge(lane);
     if (e >= 0) {
       const float x = Elem<DT>::to_float(row.p[e]);
       m = fmaxf(m, x);
       s = exp_rel(x, m);
     }
   }
-  for (int j = z * per + threadIdx.x; j < j1; j += TH * U) {
+  for (int j = z * per + lane; j < j1; j += LANES * U) {
     u32x4 w[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       w[u] = no_word<DT>();
-      if (j + u * TH < j1) w[u] = row.template word<NT>(j + u * TH);
+      if (j + u * LANES < j1) w[u] = row.template word<NT>(j + u * LANES);
     }
     hold(w);
     float x[U * W], M = m;
@@ -237,56 +241,62 @@ k_row_stats(wd_seq_rows_t q, int32_t nsplit, float2 *__restrict__ part, float2 *
     for (int i = 0; i < U * W; ++i) s += exp_rel(x[i], m);
   }
   wave_join(m, s);
-  if ((threadIdx.x & (kWave - 1)) == 0) {
-    lm[threadIdx.x / kWave] = m;
-    ls[threadIdx.x / kWave] = s;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
+  if (LANES > kWave) {
+    if ((lane & (kWave - 1)) == 0) {
+      lm[lane / kWave] = m;
+      ls[lane / kWave] = s;
+    }
+    __syncthreads();
 #pragma unroll
-    for (int w = 1; w < TH / kWave; ++w) join(m, s, lm[w], ls[w]);
+    for (int w = 1; w < LANES / kWave; ++w) join(m, s, lm[w], ls[w]);      // lane 0 holds its own wavefront's
+  }
+  if (lane == 0) {
     if (nsplit == 1) {
       stat[r] = make_float2(m, s);
-      token[r] = logp(Elem<DT>::to_float(row.p[t]), m, s);
+      token[r] = logp(xt, m, s);
     } else {
       part[r * nsplit + z] = make_float2(m, s);
+      if (z == 0) pick[r] = xt;      // whoever joins the parts may run while the gradient overwrites the logits
     }
   }
 }
 
-// the parts (a power of two, at most 64) of row r joined by as many lanes, part z in lane z of them; the first one stores (m, s) and the
-// target's log-probability and returns it
-template <int DT>
-__device__ __forceinline__ float row_join(const wd_seq_rows_t &q, int64_t r, int32_t t, int32_t nsplit, int z, const float2 *part, float2 *stat,
-                                          float *token) {
-  float2 ms = part[r * nsplit + z];
-  const float xt = Elem<DT>::to_float(((const typename Elem<DT>::type *)q.logits)[r * q.ld + t]);
-  for (int o = 1; o < nsplit; o <<= 1) join(ms.x, ms.y, __shfl_xor(ms.x, o), __shfl_xor(ms.y, o));
+// What k_row_stats leaves of rows in parts (a power of two, at most 64): (m, s) of each part and the target's logit
+struct Parts {
+  const float2 *ms;
+  const float *pick;
+  int32_t n;
+};
+// the parts of row r joined by as many lanes, part z in lane z of them; the first one stores (m, s) and the target's log-probability where
+// it is told to, and returns it
+__device__ __forceinline__ float row_join(const Parts &p, int64_t r, int z, float2 *stat, float *token) {
+  float2 ms = p.ms[r * p.n + z];
+  const float xt = p.pick[r];
+  for (int o = 1; o < p.n; o <<= 1) join(ms.x, ms.y, __shfl_xor(ms.x, o), __shfl_xor(ms.y, o));
   const float lp = logp(xt, ms.x, ms.y);
   if (z == 0) {
-    stat[r] = ms;
-    token[r] = lp;
+    if (stat) stat[r] = ms;
+    if (token) token[r] = lp;
   }
   return lp;
 }
 
 // sum and number of the actions of rows [a, b)
-template <int DT, int TH>
-__device__ __forceinline__ void seq_logp(const wd_seq_rows_t &q, int64_t a, int64_t b, int32_t nsplit, const float2 *part, float2 *stat,
-                                         float *token, double &sum, int32_t &count, double *ld, int32_t *li) {
+template <int TH>
+__device__ __forceinline__ void seq_logp(const wd_seq_rows_t &q, int64_t a, int64_t b, const Parts &p, float2 *stat, float *token,
+                                         double &sum, int32_t &count, double *ld, int32_t *li) {
   double v = 0.0;      // long sums in 64 bits: a sequence of a thousand items sums to thousands, its pair's difference to units
   int32_t c = 0;
-  if (nsplit == 1) {
+  if (p.n == 1) {
     for (int64_t r = a + threadIdx.x; r < b; r += TH) {
       v += token[r];      // 0 where the row is no action
       c += is_action(q, q.targets[r]);
     }
   } else {
-    const int z = threadIdx.x & (nsplit - 1);
-    for (int64_t r = a + threadIdx.x / nsplit; r < b; r += TH / nsplit) {      // the lanes of a row leave together
-      const int32_t t = q.targets[r];
-      if (!is_action(q, t)) continue;
-      const float lp = row_join<DT>(q, r, t, nsplit, z, part, stat, token);
+    const int z = threadIdx.x & (p.n - 1);
+    for (int64_t r = a + threadIdx.x / p.n; r < b; r += TH / p.n) {      // the lanes of a row leave together
+      if (!is_action(q, q.targets[r])) continue;
+      const float lp = row_join(p, r, z, stat, token);
       if (z == 0) {
         v += lp;
         ++c;
@@ -298,10 +308,8 @@ __device__ __forceinline__ void seq_logp(const wd_seq_rows_t &q, int64_t a, int6
 }
 
 // ---- scores: workgroup n = sequence n
-template <int DT>
 __global__ void __launch_bounds__(256)
-k_seq_logp(wd_seq_rows_t q, int32_t nsplit, int32_t length_norm, const float2 *__restrict__ part, float2 *__restrict__ stat,
-           float *__restrict__ token, float *__restrict__ seq) {
+k_seq_logp(wd_seq_rows_t q, Parts p, int32_t length_norm, float2 *__restrict__ stat, float *__restrict__ token, float *__restrict__ seq) {
   constexpr int TH = 256;
   __shared__ double ld[TH / kWave];
   __shared__ int32_t li[TH / kWave];
@@ -311,7 +319,7 @@ k_seq_logp(wd_seq_rows_t q, int32_t nsplit, int32_t length_norm, const float2 *_
   seq_range(q, n, a, b);
   double sum;
   int32_t count;
-  seq_logp<DT, TH>(q, a, b, nsplit, part, stat, token, sum, count, ld, li);
+  seq_logp<TH>(q, a, b, p, stat, token, sum, count, ld, li);
   if (threadIdx.x == 0) seq[n] = (float)(length_norm ? sum / max(count, 1) : sum);
 }
 
@@ -347,10 +355,8 @@ __device__ __forceinline__ void store_pair(const wd_pref_t &o, int64_t i, double
 }
 
 // workgroup i = pair i; leaves dloss/dlp of every row
-template <int DT>
 __global__ void __launch_bounds__(256)
-k_pref_pairs(wd_seq_rows_t q, wd_pref_t o, int32_t nsplit, const float2 *__restrict__ part, float2 *__restrict__ stat,
-             float *__restrict__ coef) {
+k_pref_pairs(wd_seq_rows_t q, wd_pref_t o, Parts p, float2 *__restrict__ stat, float *__restrict__ coef) {
   constexpr int TH = 256;
   __shared__ double ld[TH / kWave];
   __shared__ int32_t li[TH / kWave];
@@ -361,7 +367,7 @@ k_pref_pairs(wd_seq_rows_t q, wd_pref_t o, int32_t nsplit, const float2 *__restr
   int32_t n[2];
   for (int k = 0; k < 2; ++k) {
     seq_range(q, 2 * i + k, a[k], b[k]);
-    seq_logp<DT, TH>(q, a[k], b[k], nsplit, part, stat, o.token_logp, lp[k], n[k], ld, li);
+    seq_logp<TH>(q, a[k], b[k], p, stat, o.token_logp, lp[k], n[k], ld, li);
     n[k] = o.length_norm ? max(n[k], 1) : 1;
     lp[k] /= n[k];
   }
@@ -446,23 +452,23 @@ __device__ __forceinline__ void grad_part(const Row<DT> &row, typename Elem<DT>:
   }
 }
 
-template <int DT, bool NT>
+template <int DT, int LANES, bool NT>
 __global__ void __launch_bounds__(256)
 k_logits_grad(wd_seq_rows_t q, void *dlogits, int64_t ldg, int32_t zero_tail, int32_t nsplit, const float2 *__restrict__ stat,
               const float *__restrict__ coef, const float *__restrict__ pair_loss, const float *__restrict__ weights, double scale,
               float *__restrict__ loss) {
-  constexpr int TH = 256;
-  __shared__ double ld[TH / kWave];
-  const int64_t r = block_row();
+  constexpr int ROWS = 256 / LANES;
+  __shared__ double ld[256 / kWave];
   const int z = (int)blockIdx.x;
-  if (r == q.rows && z == 0 && loss) weighted_sum<TH>(pair_loss, weights, q.nseq / 2, scale, loss, ld);
+  if (loss && z == 0 && block_row() == (q.rows + ROWS - 1) / ROWS) weighted_sum<256>(pair_loss, weights, q.nseq / 2, scale, loss, ld);
+  const int64_t r = block_row() * ROWS + threadIdx.x / LANES;
   if (r >= q.rows) return;
   const bool tail = outside(q, r);
   if (tail && !zero_tail) return;
   const int32_t t = q.targets[r];
   const bool action = !tail && is_action(q, t);
   const Row<DT> row(q.logits, q.ld, r, (int)q.vocab);
-  grad_part<DT, TH, NT>(row, (typename Elem<DT>::type *)dlogits + r * ldg, z, nsplit, action, t, [&] {
+  grad_part<DT, LANES, NT>(row, (typename Elem<DT>::type *)dlogits + r * ldg, z, nsplit, action, t, [&] {
     const float2 ms = stat[r];
     return RowScalars{ms.x, ms.y, coef[r]};
   });
@@ -476,18 +482,27 @@ __device__ __forceinline__ int64_t wave_sequence(const wd_seq_rows_t &q, int64_t
   return s;
 }
 
-// small batches: pairs and gradient in one launch.  Every wavefront adds its row's pair up for itself (rows in one part, their
-// log-probabilities are there); the workgroup behind the last row does the pairs' outputs and the loss.
-__device__ __forceinline__ void wave_pair(const wd_seq_rows_t &q, const wd_pref_t &o, int64_t i, double *lp, int32_t *n) {
-  const int lane = threadIdx.x & (kWave - 1);
+// Batches of up to kPairRows rows: pairs and gradient in one launch.  Every wavefront adds its row's pair up for itself, a lane per row or
+// per part of one, behind the row's first loads; the workgroup behind the last row does the pairs' outputs and the loss.
+template <bool STORE>
+__device__ __forceinline__ void wave_pair(const wd_seq_rows_t &q, const wd_pref_t &o, int64_t i, const Parts &p, double *lp, int32_t *n) {
+  const int lane = threadIdx.x & (kWave - 1), z = lane & (p.n - 1);
   for (int k = 0; k < 2; ++k) {
     int64_t a, b;
     seq_range(q, 2 * i + k, a, b);
     double v = 0.0;
     int32_t c = 0;
-    for (int64_t r = a + lane; r < b; r += kWave) {
-      v += o.token_logp[r];
-      c += is_action(q, q.targets[r]);
+    for (int64_t r = a + lane / p.n; r < b; r += kWave / p.n) {      // the lanes of a row leave together
+      if (!is_action(q, q.targets[r])) continue;
+      float x;
+      if (p.n == 1) {
+        x = o.token_logp[r];
+      } else {
+        x = row_join(p, r, z, nullptr, STORE ? o.token_logp : nullptr);
+        if (z) continue;
+      }
+      v += x;
+      ++c;
     }
     n[k] = 1;
     if (o.length_norm) n[k] = max(wave_sum(c), 1);
@@ -495,7 +510,8 @@ __device__ __forceinline__ void wave_pair(const wd_seq_rows_t &q, const wd_pref_
   }
 }
 template <int DT>
-__global__ void __launch_bounds__(256) k_pref_grad(wd_seq_rows_t q, wd_pref_t o, int32_t nsplit, const float2 *__restrict__ stat) {
+__global__ void __launch_bounds__(256)
+k_pref_grad(wd_seq_rows_t q, wd_pref_t o, int32_t nsplit, Parts p, const float2 *__restrict__ stat) {
   constexpr int TH = 256;
   __shared__ double ld[TH / kWave];
   const int64_t r = block_row();
@@ -505,7 +521,7 @@ __global__ void __launch_bounds__(256) k_pref_grad(wd_seq_rows_t q, wd_pref_t o,
   if (r == q.rows && z == 0) {
     double total = 0.0;
     for (int64_t i = threadIdx.x / kWave; i < q.nseq / 2; i += TH / kWave) {
-      wave_pair(q, o, i, lp, n);
+      wave_pair<true>(q, o, i, p, lp, n);
       const double d = pair_difference(o, i, lp[0], lp[1]), loss = pair_loss_of(o, d);
       if (lane == 0) {
         store_pair(o, i, d, loss, lp);
@@ -522,9 +538,17 @@ __global__ void __launch_bounds__(256) k_pref_grad(wd_seq_rows_t q, wd_pref_t o,
   const bool action = !tail && is_action(q, t);
   const Row<DT> row(q.logits, q.ld, r, (int)q.vocab);
   grad_part<DT, TH, false>(row, (typename Elem<DT>::type *)o.dlogits + r * o.ld_dlogits, z, nsplit, action, t, [&] {
-    const float2 ms = stat[r];
+    float2 ms;
+    if (p.n == 1) {
+      ms = stat[r];
+    } else {
+      ms = p.ms[r * p.n + (lane & (p.n - 1))];
+      for (int k = 1; k < p.n; k <<= 1) join(ms.x, ms.y, __shfl_xor(ms.x, k), __shfl_xor(ms.y, k));
+      ms.x = __shfl(ms.x, 0);      // the sides of a join round differently
+      ms.y = __shfl(ms.y, 0);
+    }
     const int64_t s = wave_sequence(q, r);
-    wave_pair(q, o, s / 2, lp, n);
+    wave_pair<false>(q, o, s / 2, p, lp, n);
     const double slope = pair_slope(o, s / 2, pair_difference(o, s / 2, lp[0], lp[1]));
     return RowScalars{ms.x, ms.y, (float)(s & 1 ? -slope / n[1] : slope / n[0])};
   });
@@ -594,7 +618,37 @@ __device__ __forceinline__ PolicyRow policy_row(const wd_policy_t &o, float lp, 
 }
 
 // the whole row in registers between its statistics and its gradient: one read and one write of the logits, workgroup = row
-// w == nullptr: no launch has made weights and advantages; each wavefront finds them (no mean over sequences)
+// the weight of an action of sequence n, by a wavefront, for at most kSelfRows rows: a bit for each action
+__device__ __forceinline__ float self_weight(const wd_seq_rows_t &q, const wd_policy_t &o, int64_t n) {
+  if (o.reduction == WD_POLICY_SUM) return 1.f;
+  const int lane = threadIdx.x & (kWave - 1);
+  uint64_t bits[kSelfRows / kWave];
+  int32_t actions = 0;
+#pragma unroll
+  for (int k = 0; k < kSelfRows / kWave; ++k) {
+    const int64_t r = k * kWave + lane;
+    bits[k] = __ballot(r < q.rows && !outside(q, r) && is_action(q, q.targets[min(r, q.rows - 1)]));
+    actions += __popcll(bits[k]);
+  }
+  if (o.reduction == WD_POLICY_TOKEN_MEAN) return 1.0f / (float)actions;
+  auto count = [&](int64_t s) {
+    int64_t a, b;
+    seq_range(q, s, a, b);
+    int32_t c = 0;
+#pragma unroll
+    for (int k = 0; k < kSelfRows / kWave; ++k) {
+      const int lo = (int)min(max(a - k * kWave, (int64_t)0), (int64_t)kWave), hi = (int)min(max(b - k * kWave, (int64_t)0), (int64_t)kWave);
+      const uint64_t below = hi == kWave ? ~0ull : (1ull << hi) - 1, under = lo == kWave ? ~0ull : (1ull << lo) - 1;
+      c += __popcll(bits[k] & below & ~under);
+    }
+    return c;
+  };
+  int32_t seqs = 0;
+  for (int64_t s = lane; s - lane < q.nseq; s += kWave) seqs += __popcll(__ballot(s < q.nseq && count(min(s, q.nseq - 1)) > 0));
+  return (1.0f / (float)count(n)) * (1.0f / (float)seqs);
+}
+
+// w == nullptr: no launch has made weights and advantages; each wavefront finds them
 template <int DT, int TH, int NV>
 __global__ void __launch_bounds__(TH, TH == 512 ? 4 : 1)
 k_policy_resident(wd_seq_rows_t q, wd_policy_t o, const float *__restrict__ w, const float *__restrict__ adv,
@@ -636,13 +690,9 @@ k_policy_resident(wd_seq_rows_t q, wd_policy_t o, const float *__restrict__ w, c
     wr = w[r] * policy_factor(q, o, cnt);
     ar = adv[r];
   } else {
-    ar = o.advantages[o.adv_per_row ? r : wave_sequence(q, r)];
-    if (o.reduction == WD_POLICY_TOKEN_MEAN) {
-      int32_t c = 0;
-      const int64_t end = last_row(q);
-      for (int64_t i = first_row(q) + (threadIdx.x & (kWave - 1)); i < end; i += kWave) c += is_action(q, q.targets[i]);
-      wr = 1.0f / (float)wave_sum(c);
-    }
+    const int64_t n = wave_sequence(q, r);
+    ar = o.advantages[o.adv_per_row ? r : n];
+    wr = self_weight(q, o, n);
   }
   hold(v);
   float x[W], m = fmaxf(kLowest, xe);
@@ -759,6 +809,19 @@ __device__ __forceinline__ void tiny_gradient(const wd_seq_rows_t &q, const Tiny
                                 [&] { return RowScalars{x.m[r], x.s[r], x.c[r]}; });
   }
 }
+template <int DT>
+__global__ void __launch_bounds__(1024) k_seq_tiny(wd_seq_rows_t q, int32_t length_norm, float *__restrict__ token, float *__restrict__ seq) {
+  constexpr int TH = 1024;
+  __shared__ Tiny x;
+  tiny_stats<DT, TH>(q, x, token);
+  const int lane = threadIdx.x & (kWave - 1);
+  for (int n = threadIdx.x / kWave; n < q.nseq; n += TH / kWave) {      // a lane per row
+    const bool in = lane >= x.begin[n] && lane < x.end[n];
+    const double sum = wave_sum(in ? (double)x.lp[lane] : 0.0);
+    const int32_t count = wave_sum(in && x.t[lane] >= 0 ? 1 : 0);
+    if (lane == 0) seq[n] = (float)(length_norm ? sum / max(count, 1) : sum);
+  }
+}
 template <int DT> __global__ void __launch_bounds__(1024) k_pref_tiny(wd_seq_rows_t q, wd_pref_t o) {
   constexpr int TH = 1024;
   __shared__ Tiny x;
@@ -824,19 +887,17 @@ template <int DT> __global__ void __launch_bounds__(1024) k_policy_tiny(wd_seq_r
 }
 
 // rows too long for the registers: loss and coefficient of each row, a lane per part of it
-template <int DT>
 __global__ void __launch_bounds__(256)
-k_policy_join(wd_seq_rows_t q, wd_policy_t o, int32_t nsplit, const float2 *__restrict__ part, const float *__restrict__ w,
-              const float *__restrict__ adv, const int32_t *__restrict__ cnt, float2 *__restrict__ stat, float *__restrict__ coef, float *__restrict__ rows3) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, r = i / nsplit;
-  const int z = (int)(i & (nsplit - 1));
+k_policy_join(wd_seq_rows_t q, wd_policy_t o, Parts ps, const float *__restrict__ w, const float *__restrict__ adv, const int32_t *__restrict__ cnt,
+              float2 *__restrict__ stat, float *__restrict__ coef, float *__restrict__ rows3) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, r = i / ps.n;
+  const int z = (int)(i & (ps.n - 1));
   const float factor = policy_factor(q, o, cnt);      // whole wavefronts
   if (r >= q.rows) return;
   float lp = 0.f, wr = 0.f, c = 0.f;
   PolicyRow p = {0.f, 0.f, 0.f, 0.f};
-  const int32_t t = q.targets[r];
-  if (!outside(q, r) && is_action(q, t)) {
-    lp = nsplit == 1 ? o.token_logp[r] : row_join<DT>(q, r, t, nsplit, z, part, stat, o.token_logp);
+  if (!outside(q, r) && is_action(q, q.targets[r])) {
+    lp = ps.n == 1 ? o.token_logp[r] : row_join(ps, r, z, stat, o.token_logp);
     wr = w[r] * factor;
     p = policy_row(o, lp, o.old_logp[r], adv[r], o.ref_logp ? o.ref_logp[r] : 0.f);
     c = p.slope * wr * o.grad_scale;
@@ -878,8 +939,6 @@ int row_split(const wd_seq_rows_t &q) {
 // parts of a row for the gradient pass, 16 KB each: a lane has four words in flight
 int grad_split(const wd_seq_rows_t &q) { return words(q) <= 1024 ? 1 : (int)ceil_div(words(q), 1024); }
 
-// batches whose rows find their pair, weight or advantage themselves instead of in a launch of its own
-constexpr int64_t kSelfRows = 256, kSelfSeqs = 256, kPairRows = 2048;
 bool tiny(const wd_seq_rows_t &q) { return q.rows <= Tiny::kRows && q.nseq <= Tiny::kRows && q.rows * q.vocab <= 65536; }
 // whole words of the longest row that a workgroup holds in registers: 1024 lanes x 16
 constexpr int kResidentWords = 16384;
@@ -889,20 +948,22 @@ dim3 row_grid(int64_t rows, int parts) {
   return dim3((unsigned)parts, (unsigned)y, (unsigned)ceil_div(rows, y));
 }
 
-struct Work {      // [rows * nsplit] (m, s) parts | [rows] (m, s) | [rows] coefficients | 3 [rows] | [rows] weights | [rows] advantages | counts
+struct Work {      // [rows * nsplit] (m, s) parts | [rows] (m, s) | [rows] picked logits, coefficients | 3 [rows] | [rows] weights, advantages | counts
   float2 *part, *stat;
-  float *coef, *rows3, *w, *adv;
+  float *pick, *coef, *rows3, *w, *adv;
   int32_t *cnt;
   Work(const wd_seq_rows_t &q, float *p) {
     const int64_t T = q.rows;
     part = (float2 *)p;
     stat = part + T * row_split(q);
-    coef = (float *)(stat + T);
+    pick = (float *)(stat + T);
+    coef = pick + T;
     rows3 = coef + T;
     w = rows3 + 3 * T;
     adv = w + T;
     cnt = (int32_t *)(adv + T);
   }
+  Parts parts(int n) const { return {part, pick, n}; }
 };
 
 template <typename F> void by_type(int32_t dtype, F f) {
@@ -911,6 +972,8 @@ template <typename F> void by_type(int32_t dtype, F f) {
   else f(std::integral_constant<int, WD_T_BF16>());
 }
 
+// rows below 8 KB, which are never split: four to a workgroup, a wavefront each
+bool short_rows(const wd_seq_rows_t &q) { return words(q) < 512; }
 // more logits than the last cache (256 MB) holds
 bool beyond_cache(const wd_seq_rows_t &q) { return q.rows * q.ld * (q.dtype == WD_T_F32 ? 4 : 2) > ((int64_t)256 << 20); }
 
@@ -920,8 +983,9 @@ void launch_stats(const wd_seq_rows_t &q, int nsplit, const Work &k, float *toke
   by_type(q.dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const dim3 grid = row_grid(q.rows, nsplit);
-    if (!again && beyond_cache(q)) k_row_stats<DT, true><<<grid, 256, 0, st>>>(q, nsplit, k.part, k.stat, token);
-    else k_row_stats<DT, false><<<grid, 256, 0, st>>>(q, nsplit, k.part, k.stat, token);
+    if (short_rows(q)) k_row_stats<DT, kWave, false><<<row_grid(ceil_div(q.rows, 4), 1), 256, 0, st>>>(q, 1, k.part, k.pick, k.stat, token);
+    else if (!again && beyond_cache(q)) k_row_stats<DT, 256, true><<<grid, 256, 0, st>>>(q, nsplit, k.part, k.pick, k.stat, token);
+    else k_row_stats<DT, 256, false><<<grid, 256, 0, st>>>(q, nsplit, k.part, k.pick, k.stat, token);
   });
 }
 // the gradient is the last to read the logits: 1.14 GB 489 -> 448 us past the cache, 61 MB 33 -> 36 us
@@ -932,8 +996,12 @@ void launch_grad(const wd_seq_rows_t &q, int64_t rows, void *dlogits, int64_t ld
   last.rows = rows;
   const int gs = grad_split(q);
   const dim3 grid = row_grid(rows + (loss ? 1 : 0), gs);
-  if (beyond_cache(q)) k_logits_grad<DT, true><<<grid, 256, 0, st>>>(last, dlogits, ldg, zero_tail, gs, k.stat, k.coef, pair_loss, weights, scale, loss);
-  else k_logits_grad<DT, false><<<grid, 256, 0, st>>>(last, dlogits, ldg, zero_tail, gs, k.stat, k.coef, pair_loss, weights, scale, loss);
+  if (short_rows(q))
+    k_logits_grad<DT, kWave, false><<<row_grid(ceil_div(rows, 4) + (loss ? 1 : 0), 1), 256, 0, st>>>(last, dlogits, ldg, zero_tail, 1, k.stat, k.coef, pair_loss, weights, scale, loss);
+  else if (beyond_cache(q))
+    k_logits_grad<DT, 256, true><<<grid, 256, 0, st>>>(last, dlogits, ldg, zero_tail, gs, k.stat, k.coef, pair_loss, weights, scale, loss);
+  else
+    k_logits_grad<DT, 256, false><<<grid, 256, 0, st>>>(last, dlogits, ldg, zero_tail, gs, k.stat, k.coef, pair_loss, weights, scale, loss);
 }
 
 // A row in the registers of a workgroup, NV words a lane.  Two or more workgroups have to fit on a CU, so that one loads or stores while
@@ -965,7 +1033,7 @@ template <int DT> bool launch_resident(const wd_seq_rows_t &q, const wd_policy_t
 extern "C" int64_t wd_policy_workspace_floats(const wd_seq_rows_t *rows) {
   const int rc = check_rows(__func__, rows);
   if (rc) return rc;
-  return rows->rows * (2 * (int64_t)row_split(*rows) + 2 + 1 + 3 + 1 + 1) + rows->nseq + 1;
+  return rows->rows * (2 * (int64_t)row_split(*rows) + 2 + 1 + 1 + 3 + 1 + 1) + rows->nseq + 1;
 }
 
 extern "C" int wd_seq_logp(const wd_seq_rows_t *rows, int32_t length_norm, float *token_logp, float *seq_logp, float *ws,
@@ -974,12 +1042,14 @@ extern "C" int wd_seq_logp(const wd_seq_rows_t *rows, int32_t length_norm, float
   const wd_seq_rows_t q = *rows;
   WD_REQUIRE((token_logp || !q.rows) && (seq_logp || !q.nseq) && ws, "null pointer");
   hipStream_t st = as_stream(stream);
+  if (tiny(q)) {
+    by_type(q.dtype, [&](auto dt) { k_seq_tiny<decltype(dt)::value><<<1, 1024, 0, st>>>(q, length_norm, token_logp, seq_logp); });
+    return check_launch(__func__);
+  }
   const Work k(q, ws);
   const int ns = row_split(q);
   launch_stats(q, ns, k, token_logp, false, st);
-  if (q.nseq > 0) by_type(q.dtype, [&](auto dt) {
-    k_seq_logp<decltype(dt)::value><<<row_grid(q.nseq, 1), 256, 0, st>>>(q, ns, length_norm, k.part, k.stat, token_logp, seq_logp);
-  });
+  if (q.nseq > 0) k_seq_logp<<<row_grid(q.nseq, 1), 256, 0, st>>>(q, k.parts(ns), length_norm, k.stat, token_logp, seq_logp);
   return check_launch(__func__);
 }
 
@@ -1006,12 +1076,15 @@ extern "C" int wd_pref_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_pref_t *
   launch_stats(q, ns, k, o.token_logp, o.dlogits != nullptr, st);
   by_type(q.dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (ns == 1 && q.rows <= kPairRows && q.nseq <= kSelfSeqs) {
-      const int gs = (int)ceil_div(grad_split(q), 4);
-      k_pref_grad<DT><<<row_grid(q.rows + 1, gs), 256, 0, st>>>(q, o, gs, k.stat);
+    if (q.nseq <= kSelfSeqs && (q.rows <= kSelfRows || (q.rows <= kPairRows && words(q) >= 2048))) {
+      // parts of 64 KB, which make little of the pair's sums; of 16 KB where there are few rows
+      const int most = grad_split(q);
+      int gs = (int)ceil_div(most, 4);
+      if (q.rows > 0 && gs < ceil_div(2 * kCUs, q.rows)) gs = (int)(ceil_div(2 * kCUs, q.rows) < most ? ceil_div(2 * kCUs, q.rows) : most);
+      k_pref_grad<DT><<<row_grid(q.rows + 1, gs), 256, 0, st>>>(q, o, gs, k.parts(ns), k.stat);
       return;
     }
-    if (q.nseq > 0) k_pref_pairs<DT><<<row_grid(q.nseq / 2, 1), 256, 0, st>>>(q, o, ns, k.part, k.stat, k.coef);
+    if (q.nseq > 0) k_pref_pairs<<<row_grid(q.nseq / 2, 1), 256, 0, st>>>(q, o, k.parts(ns), k.stat, k.coef);
     launch_grad<DT>(q, o.dlogits ? q.rows : 0, o.dlogits, o.ld_dlogits, o.zero_tail, k, o.pair_loss, o.weights, (double)o.scale, o.loss, st);
   });
   return check_launch(__func__);
@@ -1035,7 +1108,7 @@ extern "C" int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy
   }
   Work k(q, ws);
   const int nw = words(q);
-  if (nw <= kResidentWords && q.rows <= kSelfRows && q.nseq <= kSelfSeqs && o.reduction != WD_POLICY_SEQUENCE_MEAN) k.w = nullptr;
+  if (nw <= kResidentWords && q.rows <= kSelfRows && q.nseq <= kSelfSeqs) k.w = nullptr;
   else if (q.nseq > 0) {
     if (q.rows < 256 * q.nseq) k_policy_rows<256><<<row_grid(q.nseq, 1), 256, 0, st>>>(q, o, k.w, k.adv, k.cnt);
     else k_policy_rows<1024><<<row_grid(q.nseq, 1), 1024, 0, st>>>(q, o, k.w, k.adv, k.cnt);
@@ -1047,7 +1120,7 @@ extern "C" int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy
       if (!launch_resident<DT>(q, o, k, st)) {
         const int ns = row_split(q);
         launch_stats(q, ns, k, o.token_logp, o.dlogits != nullptr, st);
-        k_policy_join<DT><<<dim3((unsigned)ceil_div(q.rows * ns, 256)), 256, 0, st>>>(q, o, ns, k.part, k.w, k.adv, k.cnt, k.stat, k.coef, k.rows3);
+        k_policy_join<<<dim3((unsigned)ceil_div(q.rows * ns, 256)), 256, 0, st>>>(q, o, k.parts(ns), k.w, k.adv, k.cnt, k.stat, k.coef, k.rows3);
         if (o.dlogits) launch_grad<DT>(q, q.rows, o.dlogits, o.ld_dlogits, o.zero_tail, k, nullptr, nullptr, 0.0, nullptr, st);
       }
     });

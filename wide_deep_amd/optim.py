@@ -58,6 +58,10 @@ class AdamW:
                 if not isinstance(t, torch.Tensor) or t.dtype not in types or t.dtype not in _DTYPES or t.shape != p.shape or t.device != dev or not t.is_contiguous():
                     raise ValueError("AdamW: %s %d: a contiguous tensor of %s like its parameter (%s on %s) is wanted, got %s" % (
                         what, k, " or ".join(map(str, types)), list(p.shape), dev, "%s %s on %s, strides %s" % (t.dtype, list(t.shape), t.device, t.stride()) if isinstance(t, torch.Tensor) else repr(t)))
+        for what, ts in (("parameters", params), ("copies", [c for c in copies if c is not None])):
+            spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in ts if t.numel())
+            if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+                raise ValueError("AdamW: %s that share memory (one tensor given twice?): every element may be updated once a step" % what)
         if dev.type != "cuda":
             raise capi.WdError("AdamW needs a GPU (MI355X / gfx950); there is no CPU fallback: parameters are on %s" % dev)
         self.params, self.grads, self.copies = params, grads, copies
@@ -95,7 +99,6 @@ class AdamW:
         self._device = dev
         self._head = (self._tensors.data_ptr(), self._chunks.data_ptr(), len(chunks), self.m.data_ptr(), second.data_ptr(), *scales,
                       self._state.data_ptr(), self._tickets.data_ptr(), 0 if self._partials is None else self._partials.data_ptr())
-        self._tail = (*self.betas,)
         self._types = (state_bits, _DTYPES[grads[0].dtype], _DTYPES[copy_type.pop()] if copy_type else 2, 0)
         self.set_step(0)
 
@@ -113,7 +116,7 @@ class AdamW:
             if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != self._device:
                 raise ValueError("AdamW.step: lr as a tensor is one fp32 value on %s, got %s %s on %s" % (self._device, lr.dtype, list(lr.shape), lr.device))
             rate, dev_rate = 0.0, lr.data_ptr()
-        self._call("wd_adamw_step", _OPTS.pack(*self._head, dev_rate, *self._tail, rate, self.eps, self.max_norm or 0.0, self.seed, *self._types))
+        self._call("wd_adamw_step", _OPTS.pack(*self._head, dev_rate, *self.betas, rate, self.eps, self.max_norm or 0.0, self.seed, *self._types))
 
     def set_step(self, step):
         """The number of steps done so far (a restored optimizer); clears `skipped`."""
@@ -135,10 +138,9 @@ class AdamW:
             raise ValueError("AdamW.moments: the moments are in `m` and `v` as they are (state_bits 32)")
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("AdamW.moments: bf16 or fp32, got %s" % dtype)
-        out = torch.empty(2, self.size, dtype=dtype, device=self._device)
-        self._call("wd_adamw_unpack", self.m.data_ptr(), self.m_scale.data_ptr(), self.r.data_ptr(), self.r_scale.data_ptr(), self.size,
-                   out[0].data_ptr(), out[1].data_ptr(), _DTYPES[dtype])
-        return out[0], out[1]
+        m, r = self.m.new_empty((2, self.size), dtype=dtype).unbind()
+        self._call("wd_adamw_unpack", self._head[3], self._head[5], self._head[4], self._head[6], self.size, m.data_ptr(), r.data_ptr(), _DTYPES[dtype])
+        return m, r
 
     def load_moments(self, m, second):
         """Flat fp32 moments of a checkpoint: m and v (state_bits 32), or m and the root of v, rounded to the nearest codes (state_bits 8)."""
