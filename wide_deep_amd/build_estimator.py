@@ -44,7 +44,7 @@ def parse_optimizer(opt, default_lr):
     if not isinstance(opt, str):
         raise ValueError("optimizer must be a string, got %r" % (opt,))
     text = opt.strip()
-    if text in _OPT_NAMES:
+    if text in _OPT_NAMES or text == "AdamW":           # AdamW: not the reference's (plan.ModelSpec.dnn_opt)
         if default_lr is None:
             raise ValueError("learning_rate must be specified when opt is supported string.")
         return text, {"learning_rate": default_lr}
@@ -58,7 +58,7 @@ def parse_optimizer(opt, default_lr):
         raise ValueError("The given object is not an Optimizer instance. Given: %s" % text)
     fn = node.func
     cls = fn.attr if isinstance(fn, ast.Attribute) else getattr(fn, "id", None)
-    if cls not in _OPT_ALIASES or not cls.endswith("Optimizer"):
+    if cls != "AdamW" and (cls not in _OPT_ALIASES or not cls.endswith("Optimizer")):
         # tf.train has no such class (AttributeError in the reference) -- or it has, and this engine does not build it
         raise _unsupported(opt)
     kwargs = {}
@@ -67,14 +67,16 @@ def parse_optimizer(opt, default_lr):
     for kw in node.keywords:
         kwargs[kw.arg] = ast.literal_eval(kw.value)
     # a constructor without learning_rate: AdamOptimizer has a default (0.001); the others require the argument
-    kwargs.setdefault("learning_rate", 0.001 if _OPT_ALIASES[cls] == "Adam" else default_lr)
-    return _OPT_ALIASES[cls], kwargs
+    name = _OPT_ALIASES.get(cls, cls)
+    kwargs.setdefault("learning_rate", 0.001 if name in ("Adam", "AdamW") else default_lr)
+    return name, kwargs
 
 
 def opt_tuple(name, kw):
     """(name, kwargs) -> the optimizer tuple of plan.ModelSpec / the oracle, with the tf.train constructor defaults:
        ("SGD", lr) ("Adagrad", lr, initial_accumulator_value) ("Ftrl", lr, l1, l2, initial_accumulator_value)
        ("RMSProp", lr, decay, momentum, epsilon) ("Adam", lr, beta1, beta2, epsilon)
+       ("AdamW", lr, beta1, beta2, epsilon, weight_decay, max_norm or None)
     Non-default variants append elements: ("Ftrl", ..., learning_rate_power) when it is not -0.5, ("Ftrl", ..., learning_rate_power,
     l2_shrinkage_regularization_strength) when the shrinkage is not 0 -- applied in the form TensorFlow >= 1.13 computes and
     its ftrl_test pins ([-0.22578995, -0.44345796] ...): the linear slot takes g + 2 shrinkage var, the accumulator the PLAIN
@@ -103,6 +105,10 @@ def opt_tuple(name, kw):
         return base + (True,) if kw.get("centered") else base
     if name == "Adam":
         return ("Adam", lr, float(kw.get("beta1", 0.9)), float(kw.get("beta2", 0.999)), float(kw.get("epsilon", 1e-8)))
+    if name == "AdamW":
+        max_norm = kw.get("max_norm")
+        return ("AdamW", lr, float(kw.get("beta1", 0.9)), float(kw.get("beta2", 0.999)), float(kw.get("epsilon", 1e-8)),
+                float(kw.get("weight_decay", 0.01)), None if max_norm is None else float(max_norm))
     raise ValueError("Unsupported optimizer: %s" % name)
 
 

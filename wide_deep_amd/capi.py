@@ -58,7 +58,7 @@ WD_CHAIN_MAX_LAYERS = 6
 WD_TN_GROUP_MAX = 20
 
 
-WD_OPT_KINDS = {"SGD": 0, "Adagrad": 1, "Ftrl": 2, "RMSProp": 3, "Adam": 4}
+WD_OPT_KINDS = {"SGD": 0, "Adagrad": 1, "Ftrl": 2, "RMSProp": 3, "Adam": 4, "AdamW": 4}      # AdamW: Adam where wd_opt_t is taken (tables)
 WD_OPT_RMSPROP_CENTERED = 6
 
 

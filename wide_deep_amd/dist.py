@@ -799,9 +799,7 @@ class ShardedWideDeepEngine(WideDeepEngine):
                 self._work_d = None
         self._collective(wait_d)
         if not self.default_opts:
-            import ctypes
-            call("wd_opt_dense", ptr(self.P), ptr(self.Pa), ptr(self.Pacc), ptr(self.G), self.P.numel(),
-                 ctypes.byref(self.opt_c["dnn_dense"]), st)
+            self._opt_dense(st)
             if self._fold_at_end():
                 self._chain_tail(capi.WD_TAIL_PACK, st)      # the MFMA-packed kernels the next tower launch reads
                 self._folded = True

@@ -62,6 +62,8 @@ class WideDeepEngine:
         for opt in ([spec.dnn_opt] if spec.has_deep else []) + ([spec.lin_opt] if spec.has_wide else []):
             if opt[0] not in capi.WD_OPT_KINDS:
                 raise ValueError("unsupported optimizer %r (supported: %s)" % (opt, sorted(capi.WD_OPT_KINDS)))
+        if spec.has_wide and spec.lin_opt[0] == "AdamW":
+            raise ValueError("AdamW is an optimizer of the dnn scope; the linear scope takes %s" % ", ".join(sorted(set(capi.WD_OPT_KINDS) - {"AdamW"})))
         # the reference's defaults (conf/model.yaml: Adagrad on the dnn scope, Ftrl on the linear scope) take the
         # specialised kernels; any other tf.train optimizer of model_util.py:84-90 the generic ones (wd_opt_t)
         self.default_opts = ((not spec.has_deep or spec.dnn_opt[0] == "Adagrad") and
@@ -239,7 +241,7 @@ class WideDeepEngine:
                 if scope == "dnn":
                     o.slot_c = self.emb_c.data_ptr()
             o.p0, o.p1, o.p2, o.p3 = opt_params(opt)
-            if opt[0] == "Adam":
+            if opt[0] in ("Adam", "AdamW"):
                 self.pow[scope] = torch.tensor([opt[2], opt[3]], **f32)
                 o.pow = self.pow[scope].data_ptr()
             self.opt_c[scope] = o
@@ -248,6 +250,7 @@ class WideDeepEngine:
         # ---- dense state -------------------------------------------------------------------
         B = self.max_batch
         self.towers = []
+        self.adamw = None
         if spec.has_deep:
             n = plan.dense_param_elems
             self.P = torch.zeros(n, **f32)
@@ -351,6 +354,8 @@ class WideDeepEngine:
                                 co[k] = pj["base"] + u * pj["pitch"] + (zoff[c] - pj["zbeg"])
                         tw["cat_off"].append(torch.from_numpy(co).to(dev))
                 self.towers.append(tw)
+            if spec.dnn_opt[0] == "AdamW":
+                self.adamw = self._make_adamw()
             self._setup_chain()
             # descriptor table of every layer of every tower (wd_fold_affine_all / wd_mlp_finalize_all)
             nl = sum(len(tw["metas"]) for tw in self.towers)
@@ -448,6 +453,47 @@ class WideDeepEngine:
     # ------------------------------------------------------------------------------------------
     # forward
     # ------------------------------------------------------------------------------------------
+    def _dense_tensors(self, buf):
+        """[(view, is a kernel)] of a buffer laid out like P: kernel, bias, gamma, beta of every layer of every tower."""
+        out = []
+        for tw in self.towers:
+            for m in tw["metas"]:
+                out.append((buf[m["w_off"]: m["w_off"] + m["K"] * m["N"]], True))
+                for k in ("b_off", "gamma_off", "beta_off"):
+                    if k in m:
+                        out.append((buf[m[k]: m[k] + m["N"]], False))
+        return out
+
+    def _make_adamw(self):
+        """dnn_opt ("AdamW", lr, beta1, beta2, epsilon, weight_decay, max_norm): one step over the tensors of P, decay on the kernels.
+        Its moments stand in buffers of its own; Pa / Pacc hold them for checkpoints (_sync_adamw)."""
+        from . import optim
+        opt = self.spec.dnn_opt
+        params = self._dense_tensors(self.P)
+        return optim.AdamW([p for p, _ in params], [g for g, _ in self._dense_tensors(self.G)], lr=opt[1], betas=(opt[2], opt[3]), eps=opt[4],
+                           weight_decay=[float(opt[5]) if kernel else 0.0 for _, kernel in params], max_norm=opt[6])
+
+    def _sync_adamw(self, load):
+        """Moments of the dense parameters: optimizer -> Pa / Pacc (what export_state reads), or back with the step count of an import."""
+        if not self.spec.has_deep or self.adamw is None:
+            return
+        for flat, buf in ((self.adamw.m, self.Pa), (self.adamw.v, self.Pacc)):
+            for start, (t, _) in zip(self.adamw.starts, self._dense_tensors(buf)):
+                part = flat[start: start + t.numel()]
+                part.copy_(t) if load else t.copy_(part)
+        if load:
+            # beta2^(t + 1) is the checkpoint's non-slot variable; at 0 (below fp32) the corrections are 1 whatever t
+            power, beta = float(self.pow["dnn"][1]), self.adamw.betas[1]
+            self.adamw.set_step(max(0, round(math.log(power) / math.log(beta)) - 1) if 0.0 < power < 1.0 and beta > 0.0 else 10 ** 6)
+
+    def _opt_dense(self, st):
+        """Any optimizer but the default Adagrad on the dense parameters of the dnn scope, gradients in G."""
+        if self.adamw is not None:
+            self.adamw.step(lr=float(self.spec.dnn_opt[1]))
+        else:
+            call("wd_opt_dense", ptr(self.P), ptr(self.Pa), ptr(self.Pacc), ptr(self.G), self.P.numel(),
+                 ctypes.byref(self.opt_c["dnn_dense"]), st)
+
     def _setup_chain(self):
         """One-launch tower (wd_tower_chain, csrc/mlp_chain.hip): exact-fp32 `simple` towers whose widths are multiples
         of 32 and whose row tile fits the LDS.  WD_CHAIN=0 keeps the per-layer GEMM launches."""
@@ -1368,8 +1414,7 @@ class WideDeepEngine:
                 call("wd_adagrad_dense", ptr(self.P), ptr(self.Pacc), ptr(self.G), self.P.numel(), float(spec.dnn_opt[1]),
                      st)
             else:
-                call("wd_opt_dense", ptr(self.P), ptr(self.Pa), ptr(self.Pacc), ptr(self.G), self.P.numel(),
-                     ctypes.byref(self.opt_c["dnn_dense"]), st)
+                self._opt_dense(st)
             if self._fold_at_end() and not (self.chain and fused_opt):   # the NEXT step's packed kernels
                 self._fold(False, st)
                 self._folded = True
@@ -1554,6 +1599,7 @@ class WideDeepEngine:
         embedding / wide tables of a 100M-row model are tens of GB; tests/helpers.compact_oracle samples their rows)."""
         plan, spec = self.plan, self.spec
         out = {}
+        self._sync_adamw(load=False)
         if spec.has_deep:
             sa, sb, sc = self._slot_bufs("dnn")
             for i, s in enumerate(plan.slots):
@@ -1601,6 +1647,7 @@ class WideDeepEngine:
 
     def import_state(self, state):
         plan, spec, dev = self.plan, self.spec, self.device
+        self._sync_adamw(load=False)      # moments the state does not hold stay what they are
         self._folded = False
         if spec.has_deep:
             sa, sb, sc = self._slot_bufs("dnn")
@@ -1646,6 +1693,7 @@ class WideDeepEngine:
             if names[0] in state:
                 self.pow[scope][0] = float(state[names[0]])
                 self.pow[scope][1] = float(state[names[1]])
+        self._sync_adamw(load=True)
         self._primed = None
         if "global_step" in state:
             self.global_step = int(state["global_step"])

@@ -119,6 +119,8 @@ class ModelSpec:
     dropout: Optional[float] = None
     # optimizer tuples (build_estimator.opt_tuple): ("SGD", lr) ("Adagrad", lr, init_accum) ("Ftrl", lr, l1, l2, init_accum)
     # ("RMSProp", lr, decay, momentum, epsilon) ("Adam", lr, beta1, beta2, epsilon)
+    # dnn_opt also ("AdamW", lr, beta1, beta2, epsilon, weight_decay, max_norm or None): optim.AdamW on the tower's parameters
+    # (weight decay on its kernels, clipping by the norm of all of them), Adam on the embedding tables
     dnn_opt: tuple = ("Adagrad", 0.05, 0.1)
     lin_opt: tuple = ("Ftrl", 0.1, 0.5, 1.0, 0.1)
     use_weight_column: bool = False
@@ -502,7 +504,7 @@ def criteo_spec(n_dense=13, n_sparse=26, buckets=1_000_000, dim=16, hidden=(256,
 # optimizer state layout (tf.train slot names; include/wd_hip.h wd_opt_t: slot a / slot b of a variable)
 # ---------------------------------------------------------------------------------------------
 OPT_SLOT_NAMES = {"SGD": (None, None), "Adagrad": (None, "/Adagrad"), "Ftrl": ("/Ftrl_1", "/Ftrl"),
-                  "RMSProp": ("/RMSProp", "/RMSProp_1"), "Adam": ("/Adam", "/Adam_1")}
+                  "RMSProp": ("/RMSProp", "/RMSProp_1"), "Adam": ("/Adam", "/Adam_1"), "AdamW": ("/Adam", "/Adam_1")}
 
 
 def ftrl_lr_power(opt):
@@ -532,7 +534,7 @@ def opt_slot_names(opt):
 # slots that are ODD functions of the gradient history (they flip sign with the parameter: a crelu layer's mirrored half
 # holds their negation), per optimizer (slot a, slot b); slot c (mean gradient) is odd
 OPT_SLOT_ODD = {"SGD": (False, False), "Adagrad": (False, False), "Ftrl": (True, False), "RMSProp": (False, True),
-                "Adam": (True, False)}
+                "Adam": (True, False), "AdamW": (True, False)}
 
 
 def opt_slot_init(opt):
@@ -547,7 +549,7 @@ def opt_slot_init(opt):
         return 0.0, float(opt[4])
     if kind == "RMSProp":
         return 1.0, 0.0           # rms slot starts at ones, momentum at zeros (RMSPropOptimizer._create_slots)
-    if kind == "Adam":
+    if kind in ("Adam", "AdamW"):
         return 0.0, 0.0
     raise ValueError("unsupported optimizer %r" % (opt,))
 
@@ -557,7 +559,7 @@ def opt_params(opt):
     kind = opt[0]
     if kind == "Ftrl":
         return float(opt[2]), float(opt[3]), ftrl_lr_power(opt), ftrl_l2_shrinkage(opt)
-    if kind in ("RMSProp", "Adam"):
+    if kind in ("RMSProp", "Adam", "AdamW"):
         return float(opt[2]), float(opt[3]), float(opt[4]), 0.0
     return 0.0, 0.0, 0.0, 0.0
 
@@ -567,7 +569,7 @@ def adam_pow_names(dnn_opt, lin_opt, has_deep, has_wide):
     then linear) owns beta1_power / beta2_power, a second Adam instance gets the _1 suffix."""
     out, n = {}, 0
     for scope, opt, on in (("dnn", dnn_opt, has_deep), ("linear", lin_opt, has_wide)):
-        if on and opt[0] == "Adam":
+        if on and opt[0] in ("Adam", "AdamW"):
             suf = "" if n == 0 else "_%d" % n
             out[scope] = ("beta1_power" + suf, "beta2_power" + suf)
             n += 1
