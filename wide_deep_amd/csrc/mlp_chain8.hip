@@ -775,7 +775,10 @@ __global__ void __launch_bounds__(NTHR, 2) k_tower_chain8(Args8 A) {
           const float a = aL[n * P + m];
           const float dbn = sdl[m] * w;
           bsum += dbn;
-          gsum += dbn * a;
+          {     // rounded product, then the sum: the order of roundings that the step has always had, not left to the compiler's choice
+#pragma clang fp contract(off)
+            gsum += dbn * a;
+          }
           const float v = dbn * sv * act_bwd(a, g.act);
           dz[n * P + m] = v;
           if (b0 + m < g.batch) wd::store1(&gdz[(b0 + m) * NL + n], v, g.flags_wt);
