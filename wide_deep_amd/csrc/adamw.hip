@@ -235,13 +235,13 @@ template <int BITS, bool WHOLE> __device__ __forceinline__ void update_piece(Pie
   for (int k = 0; k < 4; ++k) {
     const float gk = x.g[k] * h.coef;
     if (BITS == 32) {
-      x.m[k] = h.b1 * x.m[k] + h.n1 * gk;
-      x.v[k] = h.b2 * x.v[k] + h.n2 * (gk * gk);
+      x.m[k] = fmaf(h.b1, x.m[k], h.n1 * gk);
+      x.v[k] = fmaf(h.b2, x.v[k], h.n2 * (gk * gk));
       x.p[k] -= h.lr * (x.m[k] * h.c1 / (sqrtf(x.v[k]) * h.c2 + h.eps) + t.decay * x.p[k]);
-    } else {           // instructions count here: roots and reciprocals to one unit of the last place
+    } else {           // instructions count here: roots and reciprocals to one unit of the last place; rk * rk is exact (5 bits)
       const float rk = decode_r(x.rc, k, x.rs, nr);
-      x.m[k] = h.b1 * decode_m(x.mc, k, x.ms, nm) + h.n1 * gk;
-      r[k] = root_of(h.b2 * rk * rk + h.n2 * gk * gk);
+      x.m[k] = fmaf(h.b1, decode_m(x.mc, k, x.ms, nm), h.n1 * gk);
+      r[k] = root_of(fmaf(h.b2, rk * rk, h.n2 * gk * gk));
       x.p[k] -= h.lr * (x.m[k] * h.c1 * __builtin_amdgcn_rcpf(r[k] * h.c2 + h.eps) + t.decay * x.p[k]);
     }
   }
