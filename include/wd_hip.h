@@ -912,7 +912,8 @@ typedef struct wd_pref {
 int wd_pref_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_pref_t *opts, float *ws, wd_stream_t stream);
 
 /* Clipped policy loss: rho = e^(lp - old_logp[r]), A the advantage of the row or of its sequence,
- *   l = -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef k,   k = e^(ref - lp) - (ref - lp) - 1  (ref_logp NULL: 0)
+ *   l = -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef k,   k = e^(ref - lp) - (ref - lp) - 1
+ *   (ref_logp NULL: 0; kl_coef 0: k is told in sums[1] and, infinite or not, adds nothing to the loss)
  *   loss = sum_r w l;  w = 1 | 1 / actions | 1 / (sequences with an action x actions of the row's sequence)
  * sums[0..2] = loss, sum w k, sum w [the clipped side was taken]; dlogits = grad_scale dloss/dlogits (NULL: the loss alone). */
 #define WD_POLICY_SUM 0
@@ -935,7 +936,8 @@ int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy_t *opts, f
  * or in 8 bits, a half copy of the parameters) ----
  *   G = sqrt(sum g^2) over all tensors, g' = g max_norm / max(G, max_norm)            (max_norm <= 0: g' = g, G is not computed)
  *   m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;  p -= lr (m / (1 - b1^t) / (sqrt(v / (1 - b2^t)) + eps) + decay p)
- * With clipping, a step whose G is not finite changes nothing and is counted in wd_adamw_state_t.skipped.
+ * With clipping, a step whose G is not finite changes nothing and is counted in wd_adamw_state_t.skipped (squares are formed in fp32
+ * and summed in 64 bits: an element above 1.8e19 counts as not finite).  Moment buffers start at multiples of 16 bytes.
  * Moments live in flat buffers, tensor k from element tensors[k].start on (a multiple of WD_ADAMW_BLOCK; buffers as long as the
  * padded sum).  bits 32: m, v float.  bits 8: m one byte of sign, 4 exponent and 3 mantissa bits, r = sqrt(v) one byte of 4 exponent
  * and 4 mantissa bits; every block of WD_ADAMW_BLOCK values has one scale byte s, the (biased) binary exponent of its largest

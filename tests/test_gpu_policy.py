@@ -22,6 +22,7 @@ TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2
 
 class Batch:
     """Logits of ragged sequences; lengths and how many leading rows of each are no action."""
+    lanes = 256                                          # that add a row up
 
     def __init__(self, lengths, masked, vocab, dtype, seed=0, front=0, spare=0, pad=0, shift=0, spread=2.0):
         g = torch.Generator("cuda").manual_seed(seed)
@@ -53,7 +54,7 @@ class Batch:
         p = torch.softmax(z, 1)
         t = self.targets.clamp(min=0).long().unsqueeze(1)
         lp = torch.where(self.live, torch.log_softmax(z, 1).gather(1, t).squeeze(1), 0.0)
-        rs = U * (2 + 3 * (p * d.clamp(max=1e30)).sum(1) + self.V / 256 + 48)
+        rs = U * (2 + 3 * (p * d.clamp(max=1e30)).sum(1) + self.V / self.lanes + 48)
         lns = torch.logsumexp(z, 1) - m.squeeze(1)
         tol = rs + U * (d.gather(1, t).squeeze(1) + 2 * lns.abs() + lp.abs())
         return lp, p, d, torch.where(self.live, tol, 0.0), rs
@@ -336,6 +337,29 @@ def test_masks_infinities_and_lowest_values():
             q = policy.preference_loss(z[:4], t[:4], b.offs[:3])
             assert float(q.token_logp[1]) == -math.inf and float(q.difference[0]) == -math.inf and bool(q.dlogits.isfinite().all())
             assert float(q.pair_loss[0]) == math.inf
+
+
+def test_kl_that_is_only_told():
+    """kl_coef 0 with ref_logp: k is reported, and an infinite one (a reference that has not got the item's probability down) moves nothing."""
+    from wide_deep_amd import policy
+    for seqs in (1, 40):                                         # one launch, and weights from launches of their own
+        b = Batch([9] * seqs, [0] * seqs, 700, torch.float32, seed=seqs)
+        old, adv = policy.sequence_logp(b.z, b.targets, b.offs).token_logp + 0.1, b.rand(seqs)
+        ref = old.clone()
+        ref[3] = 200.0                                           # e^200 is beyond fp32
+        with_ref = policy.policy_loss(b.z, b.targets, b.offs, old, adv, ref)
+        without = policy.policy_loss(b.z, b.targets, b.offs, old, adv)
+        assert float(with_ref.kl) == math.inf and float(without.kl) == 0.0
+        assert torch.equal(with_ref.loss, without.loss) and torch.equal(with_ref.dlogits, without.dlogits) and bool(without.dlogits.isfinite().all())
+
+
+@pytest.mark.parametrize("rows,words", [(1, 2048), (1, 2049), (2, 4096), (3, 4097), (1, 8192), (1, 16384)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_few_rows_that_are_long(rows, words, dtype):
+    """Both sides of the lengths at which a handful of rows goes to one workgroup."""
+    b = Batch([1, rows - 1], [0, 0], words * (4 if dtype == "f32" else 8), DTYPES[dtype], seed=words)
+    b.lanes = 64                                                 # a wavefront adds a row up
+    check_all(b)
 
 
 def test_empty_calls_and_refusals():

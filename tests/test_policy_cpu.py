@@ -89,7 +89,7 @@ def _adamw(tensors=64, chunks=64, n=1, m=64, v=64, ms=64, rs=64, state=64, ticke
 
 
 @pytest.mark.parametrize("kw,message", [(dict(tensors=0), "null pointer"), (dict(n=0), "no chunks"), (dict(state=0), "null pointer"), (dict(tickets=0), "null pointer"), (dict(bits=16), "32 or in 8"),
-                                        (dict(bits=8, ms=0), "scales"), (dict(gt=3), "gradient type"), (dict(ct=0), "copy"), (dict(b1=1.0), "betas"),
+                                        (dict(bits=8, ms=0), "scales"), (dict(gt=3), "gradient type"), (dict(ct=0), "copy"), (dict(b1=1.0), "betas"), (dict(m=72), "aligned to 16"), (dict(v=68, bits=8), "aligned to 16"),
                                         (dict(b2=float("nan")), "betas"), (dict(eps=-1.0), "betas"), (dict(norm=1.0, partials=0), "partials")])
 def test_adamw_options_are_checked(kw, message):
     with pytest.raises(capi.WdError, match="wd_adamw_step failed .*" + message):
@@ -106,6 +106,10 @@ def test_adamw_helpers_are_checked():
         capi.call("wd_adamw_unpack", 64, 64, 64, 64, 64, 64, 64, 1, None)
     with pytest.raises(capi.WdError, match="multiple of the block"):
         capi.call("wd_adamw_pack", 64, 64, 0, 64, 64, 64, 64, None)
+    with pytest.raises(capi.WdError, match="aligned to 16"):
+        capi.call("wd_adamw_unpack", 64, 64, 64, 64, 64, 64, 72, 0, None)
+    with pytest.raises(capi.WdError, match="aligned to 16"):
+        capi.call("wd_adamw_pack", 68, 64, 64, 64, 64, 64, 64, None)
 
 
 def test_python_entry_points_refuse_before_the_device():

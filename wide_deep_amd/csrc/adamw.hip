@@ -1,7 +1,7 @@
 // wide_deep_amd/csrc/adamw.hip -- one AdamW step over many tensors, moments in 32 or in 8 bits.
 //
 // Elementwise over every parameter, so HBM bounds it: 28 bytes a parameter with 32-bit moments (p, m, v in and out, g in), 16 with 8-bit
-// ones and fp32 gradients.  One launch walks a table of 4096-element chunks of all tensors; clipping adds one pass over the gradients.
+// ones and fp32 gradients.  One launch walks a table of 2048-element chunks of all tensors; clipping adds one pass over the gradients.
 #include "common.h"
 
 namespace {
@@ -435,6 +435,7 @@ extern "C" int wd_adamw_step(const wd_adamw_t *opts, wd_stream_t stream) {
   const wd_adamw_t o = *opts;
   WD_REQUIRE(o.tensors && o.chunks && o.m && o.v && o.state && o.tickets && o.nchunks > 0, "null pointer or no chunks");
   WD_REQUIRE(o.bits == 32 || o.bits == 8, "moments are kept in 32 or in 8 bits");
+  WD_REQUIRE((((uintptr_t)o.m | (uintptr_t)o.v) & 15) == 0, "moments not aligned to 16 bytes");
   WD_REQUIRE(o.bits == 32 || (o.m_scale && o.r_scale), "8-bit moments need their scales");
   WD_REQUIRE(o.grad_dtype == WD_T_F32 || o.grad_dtype == WD_T_F16 || o.grad_dtype == WD_T_BF16, "bad gradient type");
   WD_REQUIRE(o.copy_dtype == WD_T_F16 || o.copy_dtype == WD_T_BF16, "the copy is fp16 or bf16");
@@ -458,6 +459,7 @@ extern "C" int wd_adamw_unpack(const uint8_t *m, const uint8_t *m_scale, const u
                                void *out_r, int32_t out_dtype, wd_stream_t stream) {
   WD_REQUIRE(m && m_scale && r && r_scale && out_m && out_r, "null pointer");
   WD_REQUIRE(n > 0 && n % WD_ADAMW_BLOCK == 0, "n must be a positive multiple of the block");
+  WD_REQUIRE((((uintptr_t)m | (uintptr_t)r | (uintptr_t)out_m | (uintptr_t)out_r) & 15) == 0, "buffers not aligned to 16 bytes");
   WD_REQUIRE(out_dtype == WD_T_F32 || out_dtype == WD_T_BF16, "numbers come as bf16 or fp32");
   const int64_t blocks = ceil_div(n, TH * 8);
   const int grid = (int)(blocks < 8 * kCUs ? blocks : 8 * kCUs);
@@ -470,6 +472,7 @@ extern "C" int wd_adamw_pack(const float *in_m, const float *in_r, int64_t n, ui
                              wd_stream_t stream) {
   WD_REQUIRE(in_m && in_r && m && m_scale && r && r_scale, "null pointer");
   WD_REQUIRE(n > 0 && n % WD_ADAMW_BLOCK == 0, "n must be a positive multiple of the block");
+  WD_REQUIRE((((uintptr_t)m | (uintptr_t)r | (uintptr_t)in_m | (uintptr_t)in_r) & 15) == 0, "buffers not aligned to 16 bytes");
   WD_REQUIRE(ceil_div(n, TH * 4) * TH < ((int64_t)1 << 32), "more than 2^34 values in one call");
   k_adamw_pack<<<(unsigned)ceil_div(n, TH * 4), TH, 0, as_stream(stream)>>>(in_m, in_r, n, m, m_scale, r, r_scale);
   return check_launch(__func__);
