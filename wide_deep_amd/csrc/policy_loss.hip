@@ -140,19 +140,47 @@ __device__ __forceinline__ void join(float &m, float &s, float m2, float s2) {
   m = M;
 }
 
-__device__ __forceinline__ void wave_join(float &m, float &s) {
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) join(m, s, __shfl_xor(m, o), __shfl_xor(s, o));
+// Reductions of a wavefront, the same value in every lane.  Neighbours meet inside their row of 16 lanes (each quad holds one value after the
+// first two steps, so a mirrored row is an exchange), rows by the swaps of rows and halves: no trip through LDS, 6 steps of a few cycles each (policy, odd catalogue 35.5 -> 34.3 us).
+template <typename T, typename F> __device__ __forceinline__ T by_words(T v, F f) {
+  static_assert(sizeof(T) == 4 || sizeof(T) == 8, "words");
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, f(__builtin_bit_cast(uint32_t, v)));
+  else {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(T, (uint64_t)f((uint32_t)(b >> 32)) << 32 | f((uint32_t)b));
+  }
+}
+template <int LANES> __device__ __forceinline__ auto swap_rows(uint32_t w) {
+  if constexpr (LANES == 16) return __builtin_amdgcn_permlane16_swap(w, w, false, false);
+  else return __builtin_amdgcn_permlane32_swap(w, w, false, false);
+}
+template <int CTRL, typename T> __device__ __forceinline__ T lane_move(T v) {
+  return by_words(v, [](uint32_t w) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, CTRL, 0xf, 0xf, false); });
+}
+// f of the values of lanes i and i ^ LANES, the lower one's first, in both
+template <int LANES, typename T, typename F> __device__ __forceinline__ T lane_halves(T v, F f) {
+  const auto low = by_words(v, [](uint32_t w) { return swap_rows<LANES>(w)[0]; });
+  const auto high = by_words(v, [](uint32_t w) { return swap_rows<LANES>(w)[1]; });
+  return f(low, high);
+}
+template <typename T, typename F> __device__ __forceinline__ T wave_reduce(T v, F f) {
+  v = f(v, lane_move<0xb1>(v));       // lanes 1 0 3 2 of each quad
+  v = f(v, lane_move<0x4e>(v));       // 2 3 0 1
+  v = f(v, lane_move<0x141>(v));      // half a row mirrored
+  v = f(v, lane_move<0x140>(v));      // a row mirrored
+  v = lane_halves<16>(v, f);
+  return lane_halves<32>(v, f);
 }
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
+  return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
 }
 template <typename T> __device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) v += __shfl_xor(v, o);
-  return v;
+  return wave_reduce(v, [](T a, T b) { return a + b; });
+}
+__device__ __forceinline__ void wave_join(float &m, float &s) {
+  const float M = wave_max(m);
+  s = wave_sum(s * exp_rel(m, M));
+  m = M;
 }
 // sum over the workgroup in a fixed order, the same value in every lane; `lds`: one T per wavefront, reusable after the call
 template <int TH, typename T> __device__ __forceinline__ T block_sum(T v, T *lds) {
@@ -193,13 +221,33 @@ __device__ __forceinline__ bool is_action(const wd_seq_rows_t &q, int32_t t) { r
 
 __device__ __forceinline__ float logp(float xt, float m, float s) { return (xt - m) - logf(s); }
 
+// N words into the running maximum and sum
+template <int DT, int N, int U> __device__ __forceinline__ void take_words(u32x4 (&w)[U], float &m, float &s) {
+  constexpr int W = Elem<DT>::W;
+  float x[N * W], M = m;
+#pragma unroll
+  for (int u = 0; u < N; ++u) Elem<DT>::unpack(w[u], x + u * W);
+#pragma unroll
+  for (int i = 0; i < N * W; ++i) M = fmaxf(M, x[i]);
+  s *= exp_rel(m, M);
+  m = M;
+#pragma unroll
+  for (int i = 0; i < N * W; ++i) s += exp_rel(x[i], m);
+}
+// four words of a wavefront, of which it has `left` (at least one): two that no lane has cost nothing (scores of 35 rows of 1000 bf16, replayed 7.0 -> 5.3 us)
+template <int DT> __device__ __forceinline__ void take_four(u32x4 (&w)[4], int left, float &m, float &s) {
+  hold(w);
+  if (left > 2) take_words<DT, 4>(w, m, s);
+  else take_words<DT, 2>(w, m, s);
+}
+
 // ---- (m, s) of every part of every row: LANES = 256, a workgroup a part; 64, a wavefront a (short) row.  A row in one part is done here,
 // its log-probability too.  NT: logits that the last cache cannot keep for a later pass anyway are read past it (0.39 GB: 87 -> 82 us)
 template <int DT, int LANES, bool NT>
 __global__ void __launch_bounds__(256)
 k_row_stats(wd_seq_rows_t q, int32_t nsplit, float2 *__restrict__ part, float *__restrict__ pick, float2 *__restrict__ stat,
             float *__restrict__ token) {
-  constexpr int U = 4, W = Elem<DT>::W, ROWS = 256 / LANES;
+  constexpr int U = 4, ROWS = 256 / LANES;
   __shared__ float lm[256 / kWave], ls[256 / kWave];
   const int64_t r = block_row() * ROWS + threadIdx.x / LANES;
   const int z = (int)blockIdx.x, lane = threadIdx.x & (LANES - 1);
@@ -229,16 +277,7 @@ k_row_stats(wd_seq_rows_t q, int32_t nsplit, float2 *__restrict__ part, float *_
       w[u] = no_word<DT>();
       if (j + u * LANES < j1) w[u] = row.template word<NT>(j + u * LANES);
     }
-    hold(w);
-    float x[U * W], M = m;
-#pragma unroll
-    for (int u = 0; u < U; ++u) Elem<DT>::unpack(w[u], x + u * W);
-#pragma unroll
-    for (int i = 0; i < U * W; ++i) M = fmaxf(M, x[i]);
-    s *= exp_rel(m, M);
-    m = M;
-#pragma unroll
-    for (int i = 0; i < U * W; ++i) s += exp_rel(x[i], m);
+    take_four<DT>(w, (j1 - __builtin_amdgcn_readfirstlane(j) + LANES - 1) / LANES, m, s);
   }
   wave_join(m, s);
   if (LANES > kWave) {
@@ -327,8 +366,14 @@ k_seq_logp(wd_seq_rows_t q, Parts p, int32_t length_norm, float2 *__restrict__ s
 __device__ __forceinline__ double log_sigmoid(double h) { return fmin(h, 0.0) - log1p(exp(-fabs(h))); }
 
 // ---- pairs.  The scalars of a pair are computed in 64 bits: there are a few of them, and the coefficient multiplies whole rows.
-__device__ __forceinline__ double pair_difference(const wd_pref_t &o, int64_t i, double chosen, double rejected) {
-  return chosen - rejected - (o.ref_logp ? (double)o.ref_logp[2 * i] - (double)o.ref_logp[2 * i + 1] : 0.0);
+struct PairInput {
+  float chosen, rejected, weight;      // of the reference, of the loss
+};
+__device__ __forceinline__ PairInput pair_input(const wd_pref_t &o, int64_t i) {
+  return {o.ref_logp ? o.ref_logp[2 * i] : 0.f, o.ref_logp ? o.ref_logp[2 * i + 1] : 0.f, o.weights ? o.weights[i] : 1.f};
+}
+__device__ __forceinline__ double pair_difference(const PairInput &p, double chosen, double rejected) {
+  return chosen - rejected - ((double)p.chosen - (double)p.rejected);
 }
 __device__ __forceinline__ double pair_loss_of(const wd_pref_t &o, double d) {
   if (o.kind == WD_PREF_SQUARE) {
@@ -339,8 +384,8 @@ __device__ __forceinline__ double pair_loss_of(const wd_pref_t &o, double d) {
   return -(1.0 - eps) * log_sigmoid(h) - eps * log_sigmoid(-h);
 }
 // grad_scale times dloss/dd of the batch's loss
-__device__ __forceinline__ double pair_slope(const wd_pref_t &o, int64_t i, double d) {
-  const double w = (double)o.scale * (o.weights ? (double)o.weights[i] : 1.0) * (double)o.grad_scale;
+__device__ __forceinline__ double pair_slope(const wd_pref_t &o, const PairInput &p, double d) {
+  const double w = (double)o.scale * (double)p.weight * (double)o.grad_scale;
   if (o.kind == WD_PREF_SQUARE) return 2.0 * (d - 0.5 / (double)o.beta) * w;
   // sigma(h) - (1 - eps) as eps sigma(h) - (1 - eps) sigma(-h): no cancellation where the pair is settled
   const double h = (double)o.beta * d - (double)o.margin, eps = (double)o.label_smoothing;
@@ -371,7 +416,8 @@ k_pref_pairs(wd_seq_rows_t q, wd_pref_t o, Parts p, float2 *__restrict__ stat, f
     n[k] = o.length_norm ? max(n[k], 1) : 1;
     lp[k] /= n[k];
   }
-  const double d = pair_difference(o, i, lp[0], lp[1]), slope = pair_slope(o, i, d);
+  const PairInput in = pair_input(o, i);
+  const double d = pair_difference(in, lp[0], lp[1]), slope = pair_slope(o, in, d);
   if (threadIdx.x == 0) store_pair(o, i, d, pair_loss_of(o, d), lp);
   for (int k = 0; k < 2; ++k) {
     const float c = (float)((k ? -slope : slope) / n[k]);
@@ -521,11 +567,12 @@ k_pref_grad(wd_seq_rows_t q, wd_pref_t o, int32_t nsplit, Parts p, const float2 
   if (r == q.rows && z == 0) {
     double total = 0.0;
     for (int64_t i = threadIdx.x / kWave; i < q.nseq / 2; i += TH / kWave) {
+      const PairInput in = pair_input(o, i);
       wave_pair<true>(q, o, i, p, lp, n);
-      const double d = pair_difference(o, i, lp[0], lp[1]), loss = pair_loss_of(o, d);
+      const double d = pair_difference(in, lp[0], lp[1]), loss = pair_loss_of(o, d);
       if (lane == 0) {
         store_pair(o, i, d, loss, lp);
-        total += loss * (o.weights ? (double)o.weights[i] : 1.0);
+        total += loss * (double)in.weight;
       }
     }
     total = block_sum<TH>(total, ld);
@@ -548,8 +595,9 @@ k_pref_grad(wd_seq_rows_t q, wd_pref_t o, int32_t nsplit, Parts p, const float2 
       ms.y = __shfl(ms.y, 0);
     }
     const int64_t s = wave_sequence(q, r);
+    const PairInput in = pair_input(o, s / 2);
     wave_pair<false>(q, o, s / 2, p, lp, n);
-    const double slope = pair_slope(o, s / 2, pair_difference(o, s / 2, lp[0], lp[1]));
+    const double slope = pair_slope(o, in, pair_difference(in, lp[0], lp[1]));
     return RowScalars{ms.x, ms.y, (float)(s & 1 ? -slope / n[1] : slope / n[0])};
   });
 }
@@ -744,70 +792,96 @@ k_policy_resident(wd_seq_rows_t q, wd_policy_t o, const float *__restrict__ w, c
   }
 }
 
-// ---- a handful of rows (at most 64, 64 K logits): a loss in one launch of one workgroup, a wavefront per row at a time.  The launches of
-// the general way cost a caller more than its kernels: 25 rows of 2000 14.7 -> 12.3 us a call.
+// ---- a handful of rows (at most 64, 64 K logits): a loss in one launch.  The launches of the general way cost a caller more than its kernels:
+// 25 rows of 2000 14.7 -> 12.3 us a call.  Every workgroup finds the statistics of all rows for itself, so none waits for another; they share
+// the gradient, and the first one does everything else (policy, replayed from a graph: 64 rows of 1000 15.4 -> 11.9 us, 35 rows 9.5 -> 8.6).
+// A gradient in the logits' place would be under the other workgroups' feet: one workgroup then.  Few rows are shared by wavefronts
+// (scores of one row of 65536 fp32: 24 -> 8.6 us a call; the general way 11.6).
 struct Tiny {
-  static constexpr int kRows = kWave;
+  static constexpr int kRows = kWave, kWaves = 1024 / kWave;
   float m[kRows], s[kRows], lp[kRows], c[kRows];
   int32_t t[kRows];      // the target, -1: no action
   int64_t begin[kRows], end[kRows];
+  float pm[kWaves], ps[kWaves], pt[kWaves];      // rows in parts
 };
+// wavefronts that share a row in the statistics, as a power of two; a part has 256 words or more, one round of loads
+__device__ __forceinline__ int tiny_parts(int64_t rows, int words) {
+  int p = 0;
+  while (rows << p <= Tiny::kWaves / 2 && words > 256 << p) ++p;
+  return p;
+}
+__device__ __forceinline__ int tiny_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
 template <int DT, int TH> __device__ __forceinline__ void tiny_stats(const wd_seq_rows_t &q, Tiny &x, float *token) {
-  constexpr int W = Elem<DT>::W, U = 4;
-  const int lane = threadIdx.x & (kWave - 1);
+  constexpr int U = 4;
+  const int lane = threadIdx.x & (kWave - 1), wave = tiny_wave(), shift = tiny_parts(q.rows, (int)q.vocab / Elem<DT>::W), P = 1 << shift;
+  const int z = wave & (P - 1);
   if (threadIdx.x < q.nseq) seq_range(q, threadIdx.x, x.begin[threadIdx.x], x.end[threadIdx.x]);
-  for (int64_t r = threadIdx.x / kWave; r < q.rows; r += TH / kWave) {
+  for (int r = wave >> shift; r < q.rows; r += Tiny::kWaves >> shift) {
     int32_t t = q.targets[r];
     if (outside(q, r) || !is_action(q, t)) t = -1;
-    float m = kLowest, s = 0.f, lp = 0.f;
+    float m = kLowest, s = 0.f, xt = 0.f;
     if (t >= 0) {
       const Row<DT> row(q.logits, q.ld, r, (int)q.vocab);
-      const int e = row.edge(lane);
-      const float xt = Elem<DT>::to_float(row.p[t]);
+      const int per = (row.nb + P - 1) >> shift, j1 = min(row.nb, (z + 1) * per), e = z == 0 ? row.edge(lane) : -1;
+      xt = Elem<DT>::to_float(row.p[t]);
       if (e >= 0) {
         const float v = Elem<DT>::to_float(row.p[e]);
         m = fmaxf(m, v);
         s = exp_rel(v, m);
       }
-      for (int j = lane; j < row.nb; j += kWave * U) {
+      for (int j = z * per + lane; j < j1; j += kWave * U) {
         u32x4 w[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           w[u] = no_word<DT>();
-          if (j + u * kWave < row.nb) w[u] = row.word(j + u * kWave);
+          if (j + u * kWave < j1) w[u] = row.word(j + u * kWave);
         }
-        hold(w);
-        float v[U * W], M = m;
-#pragma unroll
-        for (int u = 0; u < U; ++u) Elem<DT>::unpack(w[u], v + u * W);
-#pragma unroll
-        for (int k = 0; k < U * W; ++k) M = fmaxf(M, v[k]);
-        s *= exp_rel(m, M);
-        m = M;
-#pragma unroll
-        for (int k = 0; k < U * W; ++k) s += exp_rel(v[k], m);
+        take_four<DT>(w, (j1 - __builtin_amdgcn_readfirstlane(j) + kWave - 1) / kWave, m, s);
       }
       wave_join(m, s);
-      lp = logp(xt, m, s);
     }
     if (lane == 0) {
-      x.m[r] = m;
-      x.s[r] = s;
-      x.lp[r] = lp;
-      x.t[r] = t;
-      token[r] = lp;
+      if (z == 0) x.t[r] = t;
+      if (P > 1) {      // the rows are at most as many as there are wavefronts for
+        x.pm[wave] = m;
+        x.ps[wave] = s;
+        x.pt[wave] = xt;
+      } else {
+        x.m[r] = m;
+        x.s[r] = s;
+        x.lp[r] = t >= 0 ? logp(xt, m, s) : 0.f;
+        if (blockIdx.x == 0) token[r] = x.lp[r];
+      }
     }
   }
   __syncthreads();
+  if (P > 1) {
+    if (threadIdx.x < q.rows) {
+      const int r = threadIdx.x;
+      float m = x.pm[r * P], s = x.ps[r * P];
+      for (int k = 1; k < P; ++k) join(m, s, x.pm[r * P + k], x.ps[r * P + k]);
+      x.m[r] = m;
+      x.s[r] = s;
+      x.lp[r] = x.t[r] >= 0 ? logp(x.pt[r * P], m, s) : 0.f;
+      if (blockIdx.x == 0) token[r] = x.lp[r];
+    }
+    __syncthreads();
+  }
+}
+// and in the gradient, up to 64 of all workgroups
+__host__ __device__ __forceinline__ int tiny_grad_parts(int64_t rows, int words) {
+  return rows < 1 ? 1 : words <= 256 ? 1 : (int)(Tiny::kRows / rows) < (words + 255) / 256 ? (int)(Tiny::kRows / rows) : (words + 255) / 256;
 }
 template <int DT, int TH>
 __device__ __forceinline__ void tiny_gradient(const wd_seq_rows_t &q, const Tiny &x, void *dlogits, int64_t ldg, int32_t zero_tail) {
   __syncthreads();
   if (!dlogits) return;
-  for (int64_t r = threadIdx.x / kWave; r < q.rows; r += TH / kWave) {
+  const int P = tiny_grad_parts(q.rows, (int)q.vocab / Elem<DT>::W);
+  for (int i = blockIdx.x * Tiny::kWaves + tiny_wave(); i < q.rows * P; i += gridDim.x * Tiny::kWaves) {
+    const int r = i / P;
     if (!zero_tail && outside(q, r)) continue;
     const Row<DT> row(q.logits, q.ld, r, (int)q.vocab);
-    grad_part<DT, kWave, false>(row, (typename Elem<DT>::type *)dlogits + r * ldg, 0, 1, x.t[r] >= 0, x.t[r],
+    grad_part<DT, kWave, false>(row, (typename Elem<DT>::type *)dlogits + r * ldg, i - r * P, P, x.t[r] >= 0, x.t[r],
                                 [&] { return RowScalars{x.m[r], x.s[r], x.c[r]}; });
   }
 }
@@ -828,33 +902,43 @@ template <int DT> __global__ void __launch_bounds__(1024) k_pref_tiny(wd_seq_row
   constexpr int TH = 1024;
   __shared__ Tiny x;
   __shared__ double part[Tiny::kRows / 2];
+  const int lane = threadIdx.x & (kWave - 1), pairs = (int)q.nseq / 2;
+  PairInput next = {0.f, 0.f, 1.f};      // on its way while the rows are read
+  if (threadIdx.x / kWave < pairs) next = pair_input(o, threadIdx.x / kWave);
   tiny_stats<DT, TH>(q, x, o.token_logp);
-  const int lane = threadIdx.x & (kWave - 1);
-  for (int i = threadIdx.x / kWave; i < q.nseq / 2; i += TH / kWave) {      // a lane per row
+  for (int i = threadIdx.x / kWave; i < pairs; i += TH / kWave) {      // a lane per row
+    const PairInput in = next;
+    if (i + TH / kWave < pairs) next = pair_input(o, i + TH / kWave);
     double lp[2];
     int32_t n[2];
     for (int k = 0; k < 2; ++k) {
-      const bool in = lane >= x.begin[2 * i + k] && lane < x.end[2 * i + k];
-      n[k] = o.length_norm ? max(wave_sum(in && x.t[lane] >= 0 ? 1 : 0), 1) : 1;
-      lp[k] = wave_sum(in ? (double)x.lp[lane] : 0.0) / n[k];
+      const bool mine = lane >= x.begin[2 * i + k] && lane < x.end[2 * i + k];
+      n[k] = o.length_norm ? max(wave_sum(mine && x.t[lane] >= 0 ? 1 : 0), 1) : 1;
+      lp[k] = wave_sum(mine ? (double)x.lp[lane] : 0.0) / n[k];
     }
-    const double d = pair_difference(o, i, lp[0], lp[1]), slope = pair_slope(o, i, d), loss = pair_loss_of(o, d);
+    const double d = pair_difference(in, lp[0], lp[1]), slope = pair_slope(o, in, d), loss = pair_loss_of(o, d);
     if (lane == 0) {
-      store_pair(o, i, d, loss, lp);
-      part[i] = loss * (o.weights ? (double)o.weights[i] : 1.0);
+      if (blockIdx.x == 0) store_pair(o, i, d, loss, lp);
+      part[i] = loss * (double)in.weight;
     }
     for (int k = 0; k < 2; ++k)
       if (lane >= x.begin[2 * i + k] && lane < x.end[2 * i + k]) x.c[lane] = (float)((k ? -slope : slope) / n[k]);
   }
   tiny_gradient<DT, TH>(q, x, o.dlogits, o.ld_dlogits, o.zero_tail);
-  if (threadIdx.x < kWave) {
-    const double total = wave_sum(lane < q.nseq / 2 ? part[lane] : 0.0);
+  if (blockIdx.x == 0 && threadIdx.x < kWave) {
+    const double total = wave_sum(lane < pairs ? part[lane] : 0.0);
     if (lane == 0) *o.loss = (float)(total * (double)o.scale);
   }
 }
 template <int DT> __global__ void __launch_bounds__(1024) k_policy_tiny(wd_seq_rows_t q, wd_policy_t o) {
   constexpr int TH = 1024;
   __shared__ Tiny x;
+  float old = 0.f, ref = 0.f, adv = 0.f;      // on their way while the rows are read
+  if (threadIdx.x < q.rows) {
+    old = o.old_logp[threadIdx.x];
+    if (o.ref_logp) ref = o.ref_logp[threadIdx.x];
+  }
+  if (threadIdx.x < (o.adv_per_row ? q.rows : q.nseq)) adv = o.advantages[threadIdx.x];
   tiny_stats<DT, TH>(q, x, o.token_logp);
   if (threadIdx.x < kWave) {      // a lane per row
     const int r = threadIdx.x;
@@ -869,17 +953,18 @@ template <int DT> __global__ void __launch_bounds__(1024) k_policy_tiny(wd_seq_r
       }
       seqs += c > 0;
     }
+    if (!o.adv_per_row) adv = __shfl(adv, n);
     float loss = 0.f, kl = 0.f, clipped = 0.f;
     if (action) {
       const float w = o.reduction == WD_POLICY_SUM ? 1.0f : o.reduction == WD_POLICY_TOKEN_MEAN ? 1.0f / (float)total : (1.0f / (float)mine) * (1.0f / (float)seqs);
-      const PolicyRow p = policy_row(o, x.lp[r], o.old_logp[r], o.advantages[o.adv_per_row ? r : n], o.ref_logp ? o.ref_logp[r] : 0.f);
+      const PolicyRow p = policy_row(o, x.lp[r], old, adv, ref);
       loss = p.loss * w;
       kl = p.kl * w;
       clipped = p.clipped * w;
       x.c[r] = p.slope * w * o.grad_scale;
     }
     const double a = wave_sum((double)loss), b = wave_sum((double)kl), c = wave_sum((double)clipped);
-    if (r == 0) {
+    if (r == 0 && blockIdx.x == 0) {
       o.sums[0] = (float)a;
       o.sums[1] = (float)b;
       o.sums[2] = (float)c;
@@ -941,10 +1026,12 @@ int row_split(const wd_seq_rows_t &q) {
 // parts of a row for the gradient pass, 16 KB each: a lane has four words in flight
 int grad_split(const wd_seq_rows_t &q) { return words(q) <= 1024 ? 1 : (int)ceil_div(words(q), 1024); }
 
-// A wavefront walks a row alone, so a long row is the general way's: one of 4096 words, scores 8.4 us against 11.6, of 8192 13.4; a loss
-// with its gradient, of 2048 words 13.6 against 16.7, of 4096 18.2
-bool tiny(const wd_seq_rows_t &q, int longest) {
-  return q.rows <= Tiny::kRows && q.nseq <= Tiny::kRows && q.rows * q.vocab <= 65536 && words(q) <= longest;
+bool tiny(const wd_seq_rows_t &q) { return q.rows <= Tiny::kRows && q.nseq <= Tiny::kRows && q.rows * q.vocab <= 65536; }
+unsigned tiny_grid(const wd_seq_rows_t &q, const void *dlogits, int64_t ldg) {
+  const uintptr_t z = (uintptr_t)q.logits, g = (uintptr_t)dlogits;
+  const int64_t size = q.dtype == WD_T_F32 ? 4 : 2, nz = ((q.rows - 1) * q.ld + q.vocab) * size, ng = ((q.rows - 1) * ldg + q.vocab) * size;
+  if (!dlogits || q.rows < 1 || (z < g + ng && g < z + nz)) return 1;
+  return (unsigned)ceil_div(q.rows * tiny_grad_parts(q.rows, words(q)), Tiny::kWaves);
 }
 // whole words of the longest row that a workgroup holds in registers: 1024 lanes x 16
 constexpr int kResidentWords = 16384;
@@ -1048,7 +1135,7 @@ extern "C" int wd_seq_logp(const wd_seq_rows_t *rows, int32_t length_norm, float
   const wd_seq_rows_t q = *rows;
   WD_REQUIRE((token_logp || !q.rows) && (seq_logp || !q.nseq) && ws, "null pointer");
   hipStream_t st = as_stream(stream);
-  if (tiny(q, 4096)) {
+  if (tiny(q)) {
     by_type(q.dtype, [&](auto dt) { k_seq_tiny<decltype(dt)::value><<<1, 1024, 0, st>>>(q, length_norm, token_logp, seq_logp); });
     return check_launch(__func__);
   }
@@ -1075,8 +1162,8 @@ extern "C" int wd_pref_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_pref_t *
   hipStream_t st = as_stream(stream);
   const Work k(q, ws);
   const int ns = row_split(q);
-  if (tiny(q, 2048)) {
-    by_type(q.dtype, [&](auto dt) { k_pref_tiny<decltype(dt)::value><<<1, 1024, 0, st>>>(q, o); });
+  if (tiny(q)) {
+    by_type(q.dtype, [&](auto dt) { k_pref_tiny<decltype(dt)::value><<<tiny_grid(q, o.dlogits, o.ld_dlogits), 1024, 0, st>>>(q, o); });
     return check_launch(__func__);
   }
   launch_stats(q, ns, k, o.token_logp, o.dlogits != nullptr, st);
@@ -1108,8 +1195,8 @@ extern "C" int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy
   WD_REQUIRE(!o.dlogits || o.ld_dlogits >= q.vocab, "row stride of the gradient below the row length");
   WD_REQUIRE((uintptr_t)o.dlogits % (q.dtype == WD_T_F32 ? 4 : 2) == 0, "gradient not aligned to its element size");
   hipStream_t st = as_stream(stream);
-  if (tiny(q, 2048)) {
-    by_type(q.dtype, [&](auto dt) { k_policy_tiny<decltype(dt)::value><<<1, 1024, 0, st>>>(q, o); });
+  if (tiny(q)) {
+    by_type(q.dtype, [&](auto dt) { k_policy_tiny<decltype(dt)::value><<<tiny_grid(q, o.dlogits, o.ld_dlogits), 1024, 0, st>>>(q, o); });
     return check_launch(__func__);
   }
   Work k(q, ws);
