@@ -4,7 +4,7 @@ A graph executable that is DESTROYED while others are alive leaves the runtime w
 `hipGraphLaunch` of a live, multi-branch graph segfaults in `hip::Graph::UpdateStreams` <- `hip::GraphExec::Run`
 (profiles/r5_hipgraph_segv_backtrace.txt: the whole GPU suite in one process, the chained step graphs replayed behind ~45 tests
 whose graphs the garbage collector had destroyed; with every graph of the process kept alive the same run passes,
-profiles/r5_hipgraph_segv_pinned_graphs_pass.txt; scripts/hipgraph_segv_repro.sh reproduces both).  Nothing of ours is
+profiles/r5_hipgraph_segv_pinned_graphs_pass.txt).  Nothing of ours is
 referenced by a dead graph -- events, side streams and buffers of a capture only matter while it is replayed -- so the cure is
 on the lifetime side: every graph this package captures is registered here and lives as long as the process.  A graph
 executable is a few kernel-argument blocks (no step of ours allocates during capture: the private pool of a graph stays
@@ -26,7 +26,7 @@ _WARNED = False
 
 def new_graph():
     """torch.cuda.CUDAGraph() that is never destroyed before the process ends (WD_GRAPH_KEEPALIVE=0: an ordinary graph object,
-    destroyed with its owner -- what scripts/hipgraph_segv_repro.sh sets to show the crash)."""
+    destroyed with its owner, for a process that replays none of the others afterwards)."""
     global _WARNED
     g = torch.cuda.CUDAGraph()
     if os.environ.get("WD_GRAPH_KEEPALIVE", "1") != "0":
