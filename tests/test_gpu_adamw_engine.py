@@ -96,6 +96,16 @@ def test_learning_rates_conf_and_refusals():
     s.lin_opt = OPT
     with pytest.raises(ValueError, match="optimizer of the dnn scope"):
         WideDeepEngine(s, max_batch=64)
+    for opt in (OPT, OPT[:6] + (None,)):
+        s = _spec(opt=opt)
+        s.activation = "crelu"
+        if opt[6]:
+            with pytest.raises(ValueError, match="tied halves"):       # the norm would count a kernel twice
+                WideDeepEngine(s, max_batch=64)
+        else:
+            eng = WideDeepEngine(s, max_batch=64, seed=1)
+            eng.train_step(_batch(eng, 1))
+            assert eng.adamw.step_count == 1 and bool(eng.P.isfinite().all())
     eng = WideDeepEngine(_spec(), max_batch=64, seed=1)
     eng.set_learning_rates(dnn=0.0)
     p = eng.P.clone()

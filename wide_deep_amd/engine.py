@@ -64,6 +64,9 @@ class WideDeepEngine:
                 raise ValueError("unsupported optimizer %r (supported: %s)" % (opt, sorted(capi.WD_OPT_KINDS)))
         if spec.has_wide and spec.lin_opt[0] == "AdamW":
             raise ValueError("AdamW is an optimizer of the dnn scope; the linear scope takes %s" % ", ".join(sorted(set(capi.WD_OPT_KINDS) - {"AdamW"})))
+        if spec.has_deep and spec.dnn_opt[0] == "AdamW" and spec.dnn_opt[6] is not None and spec.activation == "crelu":
+            raise ValueError("AdamW(max_norm=...) with dnn_activation_function crelu: its layers hold every kernel twice (tied halves), so the norm of "
+                             "the gradients is not that of the variables; leave max_norm out")
         # the reference's defaults (conf/model.yaml: Adagrad on the dnn scope, Ftrl on the linear scope) take the
         # specialised kernels; any other tf.train optimizer of model_util.py:84-90 the generic ones (wd_opt_t)
         self.default_opts = ((not spec.has_deep or spec.dnn_opt[0] == "Adagrad") and
