@@ -339,6 +339,32 @@ def test_masks_infinities_and_lowest_values():
             assert float(q.pair_loss[0]) == math.inf
 
 
+@pytest.mark.parametrize("rows,seqs,vocab,dtype", [(900, 12, 5000, "bf16"), (900, 70, 3001, "f16"), (1024, 64, 600, "f32"), (1030, 64, 600, "f32"), (30, 5, 70001, "f32"), (280, 9, 140003, "f16"),
+                                                   (600, 3, 66001, "f32"), (2500, 256, 333, "bf16"), (2500, 258, 333, "bf16")])
+@pytest.mark.parametrize("reduction", ["sum", "token_mean", "sequence_mean"])
+def test_weights_that_rows_find_themselves(rows, seqs, vocab, dtype, reduction):
+    """Both sides of the sizes up to which a policy loss needs no launch for weights, rows in registers and rows too long for them."""
+    g = torch.Generator().manual_seed(rows)
+    share = torch.rand(seqs, generator=g) * (torch.rand(seqs, generator=g) < 0.8)
+    share[0] = 1.0
+    lengths = (share / share.sum() * (rows - 3)).floor().int().tolist()
+    masked = [n if k % 5 == 4 else n // 3 for k, n in enumerate(lengths)]
+    b = Batch(lengths, masked, vocab, DTYPES[dtype], seed=seqs, front=2, spare=rows - 2 - sum(lengths))
+    check_policy(b, reduction, False, 0.1)
+    check_policy(b, reduction, True, 0.0)
+    if vocab > 60000:                                            # the loss alone, and a gradient in the logits' place
+        from wide_deep_amd import policy
+        old, adv = b.reference()[0].float(), b.rand(b.N)
+        want = policy.policy_loss(b.z, b.targets, b.offs, old, adv, per_row=False, reduction=reduction)
+        alone = policy.policy_loss(b.z, b.targets, b.offs, old, adv, per_row=False, reduction=reduction, dlogits=None)
+        z = b.z.clone()
+        place = policy.policy_loss(z, b.targets, b.offs, old, adv, per_row=False, reduction=reduction, dlogits=z)
+        first, last = int(b.offs[0]), int(b.offs[-1])
+        for r in (alone, place):
+            assert torch.equal(r.loss, want.loss) and torch.equal(r.token_logp, want.token_logp)
+        assert torch.equal(z[first:last], want.dlogits[first:last])
+
+
 def test_kl_that_is_only_told():
     """kl_coef 0 with ref_logp: k is reported, and an infinite one (a reference that has not got the item's probability down) moves nothing."""
     from wide_deep_amd import policy
