@@ -365,6 +365,33 @@ def test_weights_that_rows_find_themselves(rows, seqs, vocab, dtype, reduction):
         assert torch.equal(z[first:last], want.dlogits[first:last])
 
 
+@pytest.mark.parametrize("rows,seqs,vocab,dtype", [(1024, 64, 300, "bf16"), (1025, 64, 300, "bf16"), (1024, 66, 300, "f16"), (2048, 6, 16390, "bf16"), (2049, 6, 16390, "bf16"), (2048, 2, 8193, "f32"),
+                                                   (1024, 2, 700, "f32"), (200, 64, 900, "f32"), (200, 128, 900, "f32")])
+def test_pairs_that_rows_find_themselves(rows, seqs, vocab, dtype):
+    """Both sides of the sizes up to which a preference loss needs no launch for its pairs: empty sequences, and pairs as long as the batch."""
+    from wide_deep_amd import policy
+    g = torch.Generator().manual_seed(rows)
+    share = torch.rand(seqs, generator=g) * (torch.rand(seqs, generator=g) < 0.8)
+    share[0] = 1.0
+    lengths = (share / share.sum() * (rows - 3)).floor().int().tolist()
+    masked = [n if k % 5 == 4 else n // 3 for k, n in enumerate(lengths)]
+    b = Batch(lengths, masked, vocab, DTYPES[dtype], seed=seqs, front=2, spare=rows - 2 - sum(lengths))
+    ref, w = b.rand(seqs, 3.0), torch.rand(seqs // 2, device="cuda", generator=b.g) + 0.5
+    for kind, norm in (("logistic", False), ("logistic", True), ("square", True)):
+        n = b.sums(b.live.double()).clamp(min=1) if norm else 1.0
+        near = (b.sums(b.reference()[0]) / n).float() + ref
+        want = pair_reference(b, near, w, 0.1, kind, 0.0, 0.0, norm, 1.0, 16.0)
+        r = policy.preference_loss(b.z, b.targets, b.offs, ref_logp=near, weights=w, beta=0.1, kind=kind, length_norm=norm, grad_scale=16.0)
+        for key, got in (("token", r.token_logp), ("seq", r.seq_logp), ("diff", r.difference), ("pair", r.pair_loss), ("loss", r.loss)):
+            v, t = want[key]
+            # beta, margin and scale reach the kernel as fp32: 2^-24 relative of each
+            slack = 16 * U * (v.abs() + (want["diff"][0].abs().max() + 5) * (1.0 if key == "pair" else b.N if key == "loss" else 0.0))
+            check("%s %s" % (kind, key), got, v, t + slack)
+        v, t = want["grad"]
+        own = slice(int(b.offs[0]), int(b.offs[-1]))
+        check("%s gradient" % kind, r.dlogits[own], v[own], t[own] + 16 * U * v[own].abs().amax())
+
+
 def test_kl_that_is_only_told():
     """kl_coef 0 with ref_logp: k is reported, and an infinite one (a reference that has not got the item's probability down) moves nothing."""
     from wide_deep_amd import policy

@@ -21,7 +21,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 // batches whose rows find their pair, weight or advantage themselves instead of in a launch of its own
-constexpr int64_t kSelfRows = 256, kSelfSeqs = 256, kPairRows = 2048, kWeightRows = 1024;
+constexpr int64_t kSelfRows = 256, kSelfSeqs = 256, kPairRows = 2048, kPairSeqs = 64, kWeightRows = 1024;
 static_assert(kWeightRows <= kWave * kWave, "a lane for 64 rows");
 constexpr int64_t kCountSeqs = 1024;      // up to as many sequences every wavefront adds the counts up itself
 constexpr float kLowest = -3.402823466e38f;
@@ -529,56 +529,96 @@ __device__ __forceinline__ int64_t wave_sequence(const wd_seq_rows_t &q, int64_t
   return s;
 }
 
-// Batches of up to kPairRows rows: pairs and gradient in one launch.  Every wavefront adds its row's pair up for itself, a lane per row or
+// Pairs and gradient in one launch, up to kPairRows rows and kPairSeqs sequences (self_pairs()).  Every wavefront adds its row's pair up for itself, a lane per row or
 // per part of one, behind the row's first loads; the workgroup behind the last row does the pairs' outputs and the loss.
-template <bool STORE>
 __device__ __forceinline__ void wave_pair(const wd_seq_rows_t &q, const wd_pref_t &o, int64_t i, const Parts &p, double *lp, int32_t *n) {
   const int lane = threadIdx.x & (kWave - 1), z = lane & (p.n - 1);
+  int64_t a[2], b[2];
+  for (int k = 0; k < 2; ++k) seq_range(q, 2 * i + k, a[k], b[k]);
   for (int k = 0; k < 2; ++k) {
-    int64_t a, b;
-    seq_range(q, 2 * i + k, a, b);
     double v = 0.0;
     int32_t c = 0;
-    for (int64_t r = a + lane / p.n; r < b; r += kWave / p.n) {      // the lanes of a row leave together
-      if (!is_action(q, q.targets[r])) continue;
-      float x;
-      if (p.n == 1) {
-        x = o.token_logp[r];
+    if (p.n == 1) {
+      const int first = (int)a[k] + lane, last = (int)b[k];
+      if (o.length_norm) {
+#pragma unroll 4
+        for (int r = first; r < last; r += kWave) {
+          v += o.token_logp[r];      // 0 where the row is no action
+          c += is_action(q, q.targets[r]);
+        }
       } else {
-        x = row_join(p, r, z, nullptr, STORE ? o.token_logp : nullptr);
-        if (z) continue;
+#pragma unroll 4
+        for (int r = first; r < last; r += kWave) v += o.token_logp[r];
       }
-      v += x;
-      ++c;
+    } else {
+      for (int64_t r = a[k] + lane / p.n; r < b[k]; r += kWave / p.n) {      // the lanes of a row leave together
+        if (!is_action(q, q.targets[r])) continue;
+        const float x = row_join(p, r, z, nullptr, nullptr);
+        if (z) continue;
+        v += x;
+        ++c;
+      }
     }
     n[k] = 1;
     if (o.length_norm) n[k] = max(wave_sum(c), 1);
     lp[k] = wave_sum(v) / n[k];
   }
 }
+struct PairSums {
+  double lp[kPairSeqs];
+  float token[kPairRows];
+  int32_t offs[kPairSeqs + 1];
+  uint8_t action[kPairRows];
+};
+// one workgroup: token_logp of split rows, the pairs' outputs and the loss.  All rows through LDS once, a wavefront per sequence, a lane per pair
+template <int TH> __device__ __forceinline__ void all_pairs(const wd_seq_rows_t &q, const wd_pref_t &o, const Parts &p, PairSums &x, double *ld) {
+  const int rows = (int)q.rows, seqs = (int)q.nseq, lane = threadIdx.x & (kWave - 1);
+  for (int n = threadIdx.x; n <= seqs; n += TH) x.offs[n] = min(max(q.seq_offs[n], 0), rows);
+  const int z = threadIdx.x & (p.n - 1);
+#pragma unroll 4
+  for (int r = threadIdx.x / p.n; r < rows; r += TH / p.n) {      // the lanes of a row leave together
+    const bool action = !outside(q, r) && is_action(q, q.targets[r]);
+    float lp = 0.f;
+    if (p.n == 1) lp = o.token_logp[r];
+    else if (action) lp = row_join(p, r, z, nullptr, o.token_logp);
+    if (z) continue;
+    x.token[r] = lp;
+    x.action[r] = action;
+  }
+  __syncthreads();
+  for (int n = threadIdx.x / kWave; n < seqs; n += TH / kWave) {
+    double v = 0.0;
+    int32_t c = 0;
+    for (int r = x.offs[n] + lane; r < x.offs[n + 1]; r += kWave) {
+      v += x.token[r];
+      c += x.action[r];
+    }
+    v = wave_sum(v);
+    if (o.length_norm) v /= max(wave_sum(c), 1);
+    if (lane == 0) x.lp[n] = v;
+  }
+  __syncthreads();
+  double total = 0.0;
+  for (int i = threadIdx.x; i < seqs / 2; i += TH) {
+    const PairInput in = pair_input(o, i);
+    const double d = pair_difference(in, x.lp[2 * i], x.lp[2 * i + 1]), loss = pair_loss_of(o, d);
+    store_pair(o, i, d, loss, x.lp + 2 * i);
+    total += loss * (double)in.weight;
+  }
+  total = block_sum<TH>(total, ld);
+  if (threadIdx.x == 0) *o.loss = (float)(total * (double)o.scale);
+}
 template <int DT>
 __global__ void __launch_bounds__(256)
 k_pref_grad(wd_seq_rows_t q, wd_pref_t o, int32_t nsplit, Parts p, const float2 *__restrict__ stat) {
   constexpr int TH = 256;
   __shared__ double ld[TH / kWave];
+  __shared__ PairSums sums;
   const int64_t r = block_row();
   const int z = (int)blockIdx.x, lane = threadIdx.x & (kWave - 1);
   double lp[2];
   int32_t n[2];
-  if (r == q.rows && z == 0) {
-    double total = 0.0;
-    for (int64_t i = threadIdx.x / kWave; i < q.nseq / 2; i += TH / kWave) {
-      const PairInput in = pair_input(o, i);
-      wave_pair<true>(q, o, i, p, lp, n);
-      const double d = pair_difference(in, lp[0], lp[1]), loss = pair_loss_of(o, d);
-      if (lane == 0) {
-        store_pair(o, i, d, loss, lp);
-        total += loss * (double)in.weight;
-      }
-    }
-    total = block_sum<TH>(total, ld);
-    if (threadIdx.x == 0) *o.loss = (float)(total * (double)o.scale);
-  }
+  if (r == q.rows && z == 0) all_pairs<TH>(q, o, p, sums, ld);
   if (r >= q.rows || !o.dlogits) return;
   const bool tail = outside(q, r);
   if (tail && !o.zero_tail) return;
@@ -597,7 +637,7 @@ k_pref_grad(wd_seq_rows_t q, wd_pref_t o, int32_t nsplit, Parts p, const float2 
     }
     const int64_t s = wave_sequence(q, r);
     const PairInput in = pair_input(o, s / 2);
-    wave_pair<false>(q, o, s / 2, p, lp, n);
+    wave_pair(q, o, s / 2, p, lp, n);
     const double slope = pair_slope(o, in, pair_difference(in, lp[0], lp[1]));
     return RowScalars{ms.x, ms.y, (float)(s & 1 ? -slope / n[1] : slope / n[0])};
   });
@@ -1090,6 +1130,11 @@ int self_split(const wd_seq_rows_t &q) {
   return gs;
 }
 
+// whether the rows of a preference loss find their pair themselves: a launch less, for a sum over the pair by every wavefront.  us a call with
+// and without: 1000 x 2000 in 64 sequences 13.5 / 16.4, 2000 x 30000 in 2 54 / 73, 2000 x 2000 in 4 18.2 / 15.6, 1000 x 300 in 200 24 / 16.4
+bool self_pairs(const wd_seq_rows_t &q) {
+  return q.nseq <= kPairSeqs && (q.rows <= kPairRows / 2 || (q.rows <= kPairRows && words(q) >= 2048));
+}
 // whether the rows of a policy loss find weight and advantage themselves: a launch less, for a look at every target by every wavefront.  us a call
 // with and without, 16 sequences: sum, 12000 x 300 14.8 / 17.4, 3000 x 50000 106 / 108; a mean over actions, 1000 x 8000 14.8 / 17.4,
 // 988 x 50021 43 / 37; over sequences, 1000 x 4000 14.8 / 17.3, 1000 x 8000 22 / 17.5, with 250 of them 1000 x 2000 18.8 / 17.4
@@ -1243,7 +1288,7 @@ extern "C" int wd_pref_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_pref_t *
   launch_stats(q, ns, k, o.token_logp, o.dlogits != nullptr, st);
   by_type(q.dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (q.nseq <= kSelfSeqs && (q.rows <= kSelfRows || (q.rows <= kPairRows && words(q) >= 2048))) {
+    if (self_pairs(q)) {
       const int gs = self_split(q);
       k_pref_grad<DT><<<row_grid(q.rows + 1, gs), 256, 0, st>>>(q, o, gs, k.parts(ns), k.stat);
       return;
