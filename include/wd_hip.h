@@ -943,7 +943,9 @@ int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy_t *opts, f
  * and 4 mantissa bits; every block of WD_ADAMW_BLOCK values has one scale byte s, the (biased) binary exponent of its largest
  * value, at least 27: value = code value x 2^(s - 142), code value of (e, f): (1 + f / 2^M) 2^e, e = 0: f 2^(1 - M).  A block with a value
  * that is not finite has s = 255 and reads as NaN.  Values are rounded up with the probability of their fraction, by 16 bits for
- * each moment from a hash of (flat index, step, seed): a second moment whose step is below half a code would otherwise never move. */
+ * each moment from a hash of (flat index, step, seed): a second moment whose step is below half a code would otherwise never move.
+ * A step reads code 0 of r as code 1, 2^-18 to 2^-19 of the block's largest root: elements whose root is below that take smaller steps
+ * than with 32 bits, and none of the size of m / eps. */
 #define WD_ADAMW_BLOCK 64
 #define WD_ADAMW_CHUNK 2048   /* elements of one entry of `chunks` */
 typedef struct wd_adamw_tensor {

@@ -1,0 +1,70 @@
+"""GPU: AdamW at the ends of its ranges (csrc/adamw.hip) -- blocks whose elements differ by many powers of two, limits of the norm; u = 2^-24."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BLOCK = 64
+
+
+@pytest.mark.parametrize("ratio", [1e2, 1e4, 1e5, 1e6, 1e7])
+@pytest.mark.parametrize("b2", [0.95, 0.999])
+@pytest.mark.parametrize("kind", ["steady", "spike"])
+def test_small_elements_beside_a_large_one(ratio, b2, kind):
+    """8-bit moments, one element of each block with gradients `ratio` times its neighbours', always or once.  A neighbour's root may be stored
+    as code 0 under a first moment that is not 0: the step reads code 0 as code 1, so that no update is of the size m / eps.
+
+    Each step is checked against the formula on the state as it stands (tolerance: 16 u of the update's terms, as everywhere for AdamW), and no
+    neighbour moves by more than 32 lr.  That bound: in 32 bits |m| <= K sqrt(v), K = (1 - b1) / sqrt((1 - b2)(1 - b1^2 / b2)) <= 7.3, so the
+    scale bytes are at most 3 apart; code 1 of m is then at most 2^(3 + 1) times code 1 of r, and twice that is allowed for roundings that
+    went up; the corrections' ratio is at most 2.24 where K is 1.2 (b2 0.95) and at most 1 where it is 7.3."""
+    from wide_deep_amd import optim
+    n, b1, lr, eps = 256 * BLOCK, 0.9, 1.0, 1e-8
+    gen = torch.Generator("cuda").manual_seed(int(ratio) % 1000 + 5)
+    p, g = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    opt = optim.AdamW([p], [g], lr=lr, betas=(b1, b2), eps=eps, weight_decay=0.0, state_bits=8)
+    large = torch.arange(n, device="cuda") % BLOCK == 0
+    zeros = 0
+    for t in range(1, 61):
+        g.copy_(torch.randn(n, device="cuda", generator=gen) * 1e-3)
+        if kind == "steady" or t == 10:
+            g[large] *= ratio
+        m, r = (x.double() for x in opt.moments(torch.float32))
+        zeros += int(((r == 0) & (m != 0)).sum())
+        least = torch.exp2(opt.r_scale.double() - 145.0).repeat_interleave(BLOCK)          # code 1
+        old = p.double()
+        opt.step()
+        g64 = g.double()
+        m, v = b1 * m + (1 - b1) * g64, b2 * torch.maximum(r, least) ** 2 + (1 - b2) * g64 * g64
+        size = lr / (1 - b1 ** t) / (torch.sqrt(v / (1 - b2 ** t)) + eps)
+        tol = 16 * U * size * (m.abs() + 6 / 16 * ((m - (1 - b1) * g64).abs() + (1 - b1) * g64.abs())) + U * old.abs() + 1e-45
+        off = (p.double() - (old - size * m)).abs() / tol
+        assert float(off.max()) <= 1.0, (t, float(off.max()))
+        assert float((p.double() - old)[~large].abs().max()) <= 32 * lr, t
+    assert zeros > 0 or ratio < 1e5 or (kind == "spike" and ratio < 1e6)                   # the cases that matter were met
+
+
+def test_loaded_roots_of_code_zero():
+    """Numbers of a checkpoint far below their block's largest root: loaded to nearest they are code 0, and the next step stays bounded."""
+    from wide_deep_amd import optim
+    n = 4 * BLOCK
+    p, g = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    opt = optim.AdamW([p], [g], lr=1.0, weight_decay=0.0, state_bits=8)
+    m, r = torch.full((n,), 1e-3, device="cuda"), torch.full((n,), 1e-3, device="cuda")
+    r[::BLOCK] = 1e4
+    opt.load_moments(m, r)
+    opt.set_step(1000)
+    assert int((opt.r == 0).sum()) == n - n // BLOCK
+    opt.step()
+    # code 1 is 2^-18 of 2^13 <= 1e4: the update is 0.9e-3 / (2^-5 sqrt(0.999) / sqrt(1 - 0.999^1001)) = 0.023
+    want = 0.9e-3 / (2.0 ** -5 * math.sqrt(0.999 / (1 - 0.999 ** 1001)))
+    # m was rounded to a code: half a step of 3 bits
+    assert abs(float(p[1]) + want) <= want / 16 + 1e-6 and bool((p.abs() <= 0.03).all())
+    # a block that holds nothing but zeros still holds nothing
+    opt.load_moments(torch.zeros_like(m), torch.zeros_like(r))
+    p.zero_()
+    opt.step()
+    assert bool((p == 0).all()) and bool((opt.r == 0).all())
