@@ -1,0 +1,54 @@
+"""GPU: what the policy heads answer where a log-probability, a ratio or a difference is infinite (csrc/policy_loss.hip), and losses without a
+gradient, each in every way that the launches take."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+# rows, vocab, type: a handful in one launch, short rows, rows split over workgroups, many sequences, rows longer than the registers
+SHAPES = [(8, 100, "f32"), (400, 300, "bf16"), (40, 9001, "f32"), (3000, 501, "f16"), (2600, 40, "f32"), (40, 140003, "bf16"), (1500, 66001, "f32")]
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def make(rows, vocab, dtype, seqs=4, seed=0):
+    """Logits, targets, offsets of `seqs` sequences of equal length; row 1 of the second sequence has an item that cannot be chosen, and it was."""
+    g = torch.Generator("cuda").manual_seed(rows + vocab + seed)
+    z = torch.randn(rows, vocab, device="cuda", generator=g).to(DTYPES[dtype])
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    per = rows // seqs
+    offs = torch.arange(seqs + 1, device="cuda", dtype=torch.int32) * per
+    bad = per + 1
+    z[bad, int(t[bad])] = -math.inf
+    return z, t, offs, bad
+
+
+def several(rows):
+    return 4 if rows < 2600 else 4 if rows == 3000 else 1300
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", SHAPES)
+@pytest.mark.parametrize("norm", [False, True])
+def test_a_rejected_sequence_that_cannot_be(rows, vocab, dtype, norm):
+    """d = +inf: the pair is settled, its loss is 0 (label_smoothing 0) and it moves nothing; with smoothing the loss is +inf, the slope beta eps."""
+    from wide_deep_amd import policy
+    z, t, offs, bad = make(rows, vocab, dtype, several(rows))
+    a, b, c = offs[:3].tolist()
+    w = torch.full((len(offs) // 2,), 0.5, device="cuda")
+    for margin in (0.0, 0.25):
+        r = policy.preference_loss(z, t, offs, weights=w, margin=margin, length_norm=norm)
+        assert float(r.token_logp[bad]) == -math.inf and float(r.seq_logp[1]) == -math.inf and float(r.difference[0]) == math.inf
+        assert float(r.pair_loss[0]) == 0.0 and bool(r.pair_loss.isfinite().all())
+        want = float((r.pair_loss.double() * 0.5).sum())
+        assert abs(float(r.loss) - want) <= 2.0 ** -22 * want + 2.0 ** -24 * float(r.pair_loss.double().sum())      # pair_loss and loss round once each
+        assert bool((r.dlogits[a:c] == 0).all()) and bool(r.dlogits.isfinite().all()) and bool((r.dlogits[c:] != 0).any())
+    smooth = policy.preference_loss(z, t, offs, label_smoothing=0.1, length_norm=norm)
+    assert float(smooth.pair_loss[0]) == math.inf and float(smooth.loss) == math.inf and bool(smooth.dlogits.isfinite().all())
+    # the other way round: the chosen one cannot be
+    t2 = t.clone()
+    z2 = z.clone()
+    z2[bad] = z[bad].nan_to_num(0.0, neginf=0.0)
+    z2[1, int(t[1])] = -math.inf
+    r = policy.preference_loss(z2, t2, offs, length_norm=norm)
+    assert float(r.difference[0]) == -math.inf and float(r.pair_loss[0]) == math.inf and bool(r.dlogits.isfinite().all())

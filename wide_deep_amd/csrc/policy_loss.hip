@@ -382,7 +382,8 @@ __device__ __forceinline__ double pair_loss_of(const wd_pref_t &o, double d) {
     return h * h;
   }
   const double h = (double)o.beta * d - (double)o.margin, eps = (double)o.label_smoothing;
-  return -(1.0 - eps) * log_sigmoid(h) - eps * log_sigmoid(-h);
+  const double loss = -(1.0 - eps) * log_sigmoid(h);
+  return eps > 0.0 ? loss - eps * log_sigmoid(-h) : loss;      // a pair that is settled for good, h = inf: 0 x inf is no loss
 }
 // grad_scale times dloss/dd of the batch's loss
 __device__ __forceinline__ double pair_slope(const wd_pref_t &o, const PairInput &p, double d) {
