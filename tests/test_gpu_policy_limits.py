@@ -52,3 +52,30 @@ def test_a_rejected_sequence_that_cannot_be(rows, vocab, dtype, norm):
     z2[1, int(t[1])] = -math.inf
     r = policy.preference_loss(z2, t2, offs, length_norm=norm)
     assert float(r.difference[0]) == -math.inf and float(r.pair_loss[0]) == math.inf and bool(r.dlogits.isfinite().all())
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", SHAPES)
+@pytest.mark.parametrize("reduction", ["sum", "token_mean", "sequence_mean"])
+def test_kl_of_an_item_that_cannot_be(rows, vocab, dtype, reduction):
+    """token_logp = -inf under a reference that could choose the item: k = e^inf - inf - 1 = +inf; with kl_coef 0 it is told and moves nothing."""
+    from wide_deep_amd import policy
+    z, t, offs, bad = make(rows, vocab, dtype, several(rows))
+    ref = policy.sequence_logp(z, t, offs).token_logp.clone()
+    assert float(ref[bad]) == -math.inf
+    ref[bad] = -3.0
+    adv = torch.ones(len(offs) - 1, device="cuda")
+    call = lambda **kw: policy.policy_loss(z, t, offs, ref, adv, per_row=False, reduction=reduction, **kw)
+    told, without, alone = call(ref_logp=ref), call(), call(ref_logp=ref, dlogits=None)
+    for r in (told, alone):
+        assert float(r.kl) == math.inf and torch.equal(r.loss, without.loss) and bool(r.loss.isfinite())
+    assert torch.equal(told.dlogits, without.dlogits) and bool(told.dlogits.isfinite().all()) and bool((told.dlogits[bad] == 0).all())
+    taken = call(ref_logp=ref, kl_coef=0.1)
+    others = torch.arange(rows, device="cuda") != bad
+    assert float(taken.kl) == math.inf and float(taken.loss) == math.inf and bool(taken.dlogits[others].isfinite().all())
+    # a reference that could not choose the item either side of it: k = e^-inf + inf - 1
+    far = ref.clone()
+    far[bad + 1] = -math.inf
+    z2 = z.clone()
+    z2[bad] = z[bad].nan_to_num(0.0, neginf=0.0)
+    r = policy.policy_loss(z2, t, offs, ref, adv, ref_logp=far, per_row=False, reduction=reduction, kl_coef=0.1)
+    assert float(r.kl) == math.inf and float(r.loss) == math.inf and bool(r.dlogits.isfinite().all())

@@ -700,7 +700,7 @@ __device__ __forceinline__ PolicyRow policy_row(const wd_policy_t &o, float lp, 
   p.kl = 0.f;
   if (o.ref_logp) {
     const float d = ref - lp, e = expm1f(d);
-    p.kl = e - d;
+    p.kl = e == INFINITY ? e : e - d;      // lp = -inf: d is infinite too, e^d the larger
     if (o.kl_coef != 0.f) {      // told of only: an infinite k leaves the loss alone
       p.loss += o.kl_coef * p.kl;
       p.slope -= o.kl_coef * e;
