@@ -79,3 +79,33 @@ def test_kl_of_an_item_that_cannot_be(rows, vocab, dtype, reduction):
     z2[bad] = z[bad].nan_to_num(0.0, neginf=0.0)
     r = policy.policy_loss(z2, t, offs, ref, adv, ref_logp=far, per_row=False, reduction=reduction, kl_coef=0.1)
     assert float(r.kl) == math.inf and float(r.loss) == math.inf and bool(r.dlogits.isfinite().all())
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", SHAPES)
+@pytest.mark.parametrize("clip", [(0.2, 0.2), (1.0, math.inf)])
+def test_an_advantage_of_zero_tells_nothing_whatever_the_ratio(rows, vocab, dtype, clip):
+    """rho = e^(lp - old) above fp32 (old far below, or -inf): 0 x inf is no loss and no slope.  With another advantage it stays what it was."""
+    from wide_deep_amd import policy
+    z, t, offs, bad = make(rows, vocab, dtype, several(rows))
+    z[bad] = z[bad].nan_to_num(0.0, neginf=0.0)
+    lp = policy.sequence_logp(z, t, offs).token_logp
+    old, adv = lp - 0.05, torch.ones(rows, device="cuda")
+    for far in (lp[1] - 100.0, torch.tensor(-math.inf)):
+        old[1], adv[1] = far, 0.0
+        for zero in (0.0, -0.0):
+            adv[1] = zero
+            r = policy.policy_loss(z, t, offs, old, adv, per_row=True, clip=clip, reduction="sum")
+            near = old.clone()
+            near[1] = lp[1]
+            want = policy.policy_loss(z, t, offs, near, adv, per_row=True, clip=clip, reduction="sum")
+            assert torch.equal(r.loss, want.loss) and torch.equal(r.clipped, want.clipped) and bool((r.dlogits[1] == 0).all())
+            assert torch.equal(r.dlogits, want.dlogits)
+            alone = policy.policy_loss(z, t, offs, old, adv, per_row=True, clip=clip, reduction="sum", dlogits=None)
+            assert torch.equal(alone.loss, want.loss)
+        adv[1] = -1.0
+        r = policy.policy_loss(z, t, offs, old, adv, per_row=True, clip=clip, reduction="sum")
+        assert float(r.loss) == math.inf
+        if clip[1] < 1.0:
+            adv[1] = 1.0
+            r = policy.policy_loss(z, t, offs, old, adv, per_row=True, clip=clip, reduction="sum")
+            assert bool(r.loss.isfinite()) and bool((r.dlogits[1] == 0).all()) and float(r.clipped) == 1.0

@@ -692,7 +692,8 @@ struct PolicyRow {
 __device__ __forceinline__ PolicyRow policy_row(const wd_policy_t &o, float lp, float old, float adv, float ref) {
   PolicyRow p;
   const float rho = expf(lp - old);
-  const float a = rho * adv, b = fminf(fmaxf(rho, 1.0f - o.clip_low), 1.0f + o.clip_high) * adv;
+  const float a = adv == 0.f && rho == INFINITY ? 0.f : rho * adv;      // no advantage: no loss and no slope, also where the ratio is beyond fp32
+  const float b = fminf(fmaxf(rho, 1.0f - o.clip_low), 1.0f + o.clip_high) * adv;
   const bool out = a > b;
   p.loss = -(out ? b : a);
   p.slope = out ? 0.f : -a;
