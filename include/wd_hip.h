@@ -892,7 +892,7 @@ int wd_seq_logp(const wd_seq_rows_t *rows, int32_t length_norm, float *token_log
  *   d = (LP[2i] - ref[2i]) - (LP[2i + 1] - ref[2i + 1])
  *   LOGISTIC  h = beta d - margin;  pair_loss = -(1 - eps) log sigma(h) - eps log sigma(-h)
  *   SQUARE    pair_loss = (d - 1 / (2 beta))^2          (no margin, no smoothing)
- *   loss = scale sum_i weights[i] pair_loss[i]
+ *   loss = scale sum_i weights[i] pair_loss[i]          (a pair of weight 0 adds nothing, whatever its loss)
  * and dlogits = grad_scale dloss/dlogits (NULL: the loss alone). */
 #define WD_PREF_LOGISTIC 0
 #define WD_PREF_SQUARE 1

@@ -109,3 +109,21 @@ def test_an_advantage_of_zero_tells_nothing_whatever_the_ratio(rows, vocab, dtyp
             adv[1] = 1.0
             r = policy.policy_loss(z, t, offs, old, adv, per_row=True, clip=clip, reduction="sum")
             assert bool(r.loss.isfinite()) and bool((r.dlogits[1] == 0).all()) and float(r.clipped) == 1.0
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", SHAPES)
+@pytest.mark.parametrize("kind", ["logistic", "square"])
+def test_pairs_of_weight_zero_add_nothing(rows, vocab, dtype, kind):
+    """A pair left out by its weight is left out, an infinite loss of its own is told in pair_loss and nowhere else."""
+    from wide_deep_amd import policy
+    z, t, offs, bad = make(rows, vocab, dtype, several(rows))
+    a, b, c = offs[:3].tolist()
+    z[bad] = z[bad].nan_to_num(0.0, neginf=0.0)
+    z[1, int(t[1])] = -math.inf                              # the chosen sequence of the first pair cannot be
+    w = torch.full((len(offs) // 2,), 0.5, device="cuda")
+    w[0] = 0.0
+    r = policy.preference_loss(z, t, offs, weights=w, kind=kind)
+    assert float(r.difference[0]) == -math.inf and float(r.pair_loss[0]) == math.inf
+    want = float((r.pair_loss[1:].double() * 0.5).sum())
+    assert abs(float(r.loss) - want) <= 2.0 ** -23 * want      # pair_loss and loss round once each
+    assert bool((r.dlogits[a:c] == 0).all()) and bool(r.dlogits.isfinite().all()) and bool((r.dlogits[c:] != 0).any())

@@ -385,8 +385,11 @@ __device__ __forceinline__ double pair_loss_of(const wd_pref_t &o, double d) {
   const double loss = -(1.0 - eps) * log_sigmoid(h);
   return eps > 0.0 ? loss - eps * log_sigmoid(-h) : loss;      // a pair that is settled for good, h = inf: 0 x inf is no loss
 }
+// what a pair adds to the sum of the batch's loss
+__device__ __forceinline__ double weighted(double loss, double weight) { return weight == 0.0 ? 0.0 : loss * weight; }
 // grad_scale times dloss/dd of the batch's loss
 __device__ __forceinline__ double pair_slope(const wd_pref_t &o, const PairInput &p, double d) {
+  if (p.weight == 0.f) return 0.0;      // a pair that is left out adds nothing, an infinite d of its own too
   const double w = (double)o.scale * (double)p.weight * (double)o.grad_scale;
   if (o.kind == WD_PREF_SQUARE) return 2.0 * (d - 0.5 / (double)o.beta) * w;
   // sigma(h) - (1 - eps) as eps sigma(h) - (1 - eps) sigma(-h): no cancellation where the pair is settled
@@ -440,7 +443,7 @@ template <int TH> __device__ __forceinline__ void weighted_sum(const float *v, c
       y[u] = in && w ? w[i + u * TH] : 1.f;
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) t += (double)x[u] * (double)y[u];
+    for (int u = 0; u < U; ++u) t += weighted((double)x[u], (double)y[u]);
   }
   t = block_sum<TH>(t, ld);
   if (threadIdx.x == 0) *out = (float)(t * scale);
@@ -604,7 +607,7 @@ template <int TH> __device__ __forceinline__ void all_pairs(const wd_seq_rows_t 
     const PairInput in = pair_input(o, i);
     const double d = pair_difference(in, x.lp[2 * i], x.lp[2 * i + 1]), loss = pair_loss_of(o, d);
     store_pair(o, i, d, loss, x.lp + 2 * i);
-    total += loss * (double)in.weight;
+    total += weighted(loss, (double)in.weight);
   }
   total = block_sum<TH>(total, ld);
   if (threadIdx.x == 0) *o.loss = (float)(total * (double)o.scale);
@@ -970,7 +973,7 @@ template <int DT> __global__ void __launch_bounds__(1024) k_pref_tiny(wd_seq_row
     const double d = pair_difference(in, lp[0], lp[1]), slope = pair_slope(o, in, d), loss = pair_loss_of(o, d);
     if (lane == 0) {
       if (blockIdx.x == 0) store_pair(o, i, d, loss, lp);
-      part[i] = loss * (double)in.weight;
+      part[i] = weighted(loss, (double)in.weight);
     }
     for (int k = 0; k < 2; ++k)
       if (lane >= x.begin[2 * i + k] && lane < x.end[2 * i + k]) x.c[lane] = (float)((k ? -slope : slope) / n[k]);

@@ -120,7 +120,7 @@ def preference_loss(logits, targets, seq_offs, ref_logp=None, weights=None, beta
 
     d = (LP[2i] - ref_logp[2i]) - (LP[2i + 1] - ref_logp[2i + 1]) with LP as seq_logp of sequence_logp (which also makes ref_logp, from
     the reference model's logits); kind "logistic": -(1 - label_smoothing) log sigma(h) - label_smoothing log sigma(-h), h = beta d -
-    margin; "square": (d - 1 / (2 beta))^2.  loss = sum or mean over the pairs of weights[i] times that.
+    margin; "square": (d - 1 / (2 beta))^2.  loss = sum or mean over the pairs of weights[i] times that (a pair of weight 0 adds nothing, whatever its loss).
     dlogits: True (a new tensor), a tensor like logits (rows of no sequence are left as they were; it may be `logits` itself), or None
     (the loss alone); it holds grad_scale times the gradient."""
     rows, T, V, N, dev, code = _rows(logits, targets, seq_offs)
