@@ -934,7 +934,7 @@ int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy_t *opts, f
 
 /* ---- AdamW over many tensors at once (beside wd_opt_dense: decoupled decay per tensor, clipping by the global norm, moments in 32
  * or in 8 bits, a half copy of the parameters) ----
- *   G = sqrt(sum g^2) over all tensors, g' = g max_norm / max(G, max_norm)            (max_norm <= 0: g' = g, G is not computed)
+ *   G = sqrt(sum g^2) over all tensors, g' = g max_norm / max(G, max_norm)            (max_norm <= 0: g' = g, G is not computed; infinite: g' = g)
  *   m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;  p -= lr (m / (1 - b1^t) / (sqrt(v / (1 - b2^t)) + eps) + decay p)
  * With clipping, a step whose G is not finite changes nothing and is counted in wd_adamw_state_t.skipped (squares are formed in fp32
  * and summed in 64 bits: an element above 1.8e19 counts as not finite).  Moment buffers start at multiples of 16 bytes.

@@ -68,3 +68,36 @@ def test_loaded_roots_of_code_zero():
     p.zero_()
     opt.step()
     assert bool((p == 0).all()) and bool((opt.r == 0).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_infinite_max_norm_only_tells_the_norm(bits):
+    from wide_deep_amd import optim
+    sizes = [5, 64, 4099]
+
+    def run(max_norm):
+        gen = torch.Generator("cuda").manual_seed(3)
+        p = [torch.randn(n, device="cuda", generator=gen) for n in sizes]
+        g = [torch.randn(n, device="cuda", generator=gen) for n in sizes]
+        opt = optim.AdamW(p, g, max_norm=max_norm, state_bits=bits)
+        for _ in range(3):
+            opt.step()
+        return opt
+
+    a, b = run(None), run(math.inf)
+    assert all(torch.equal(x, y) for x, y in zip(a.params + [a.m], b.params + [b.m])) and all(bool(x.isfinite().all()) for x in b.params)
+    norm = math.sqrt(sum(float(g.double().square().sum()) for g in b.grads))
+    assert abs(float(b.grad_norm) - norm) <= 10 * U * norm and b.step_count == 3 and b.skipped == 0
+    b.grads[1][3] = math.inf
+    b.step()
+    assert b.skipped == 1 and all(torch.equal(x, y) for x, y in zip(a.params, b.params))
+
+
+def test_a_max_norm_that_is_no_fp32_number_is_refused():
+    """2^-150 reaches the kernel as 0, which means no clipping."""
+    from wide_deep_amd import optim
+    p, g = [torch.zeros(4, device="cuda")], [torch.zeros(4, device="cuda")]
+    for bad in (0.0, -1.0, 2.0 ** -151, math.nan):
+        with pytest.raises(ValueError, match="max_norm"):
+            optim.AdamW(p, g, max_norm=bad)
+    optim.AdamW(p, g, max_norm=2.0 ** -149).step()

@@ -322,7 +322,7 @@ k_adamw(wd_adamw_t o, const wd_adamw_tensor_t *__restrict__ tensors, const int32
     const double G = sqrt(block_sum(s, lds));
     norm = (float)G;
     skip = !(G < (double)INFINITY);
-    h.coef = (float)((double)o.max_norm / fmax(G, (double)o.max_norm));
+    h.coef = G > (double)o.max_norm ? (float)((double)o.max_norm / G) : 1.f;      // max_norm may be infinite: the norm is told, nothing clipped
   }
   // backwards: the norm's pass has left the ends of the gradients in the last cache
   int64_t c = o.nchunks - 1 - blockIdx.x;

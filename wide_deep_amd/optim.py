@@ -21,7 +21,7 @@ _OPTS = struct.Struct("=QQqQQQQQQQQddfffIiiii")     # wd_adamw_t
 
 class AdamW:
     """params, grads: lists of contiguous tensors on one GPU, fp32 and fp32 / fp16 / bf16 (one type for all gradients), bound for good.
-    weight_decay: one number or one per tensor.  max_norm: clip by the global norm of all gradients; a step whose norm is not finite
+    weight_decay: one number or one per tensor.  max_norm: clip by the global norm of all gradients (math.inf: tell it and clip nothing); a step whose norm is not finite
     (an element above 1.8e19, too: its square is formed in fp32) changes nothing and is counted in `skipped`.  state_bits: 32, or 8 (m and the root r of the second moment, one byte each; rounding by
     a hash of index, step and `seed`, so runs repeat; elements whose root is below 2^-18 of the largest of their 64 take smaller steps than with 32).  copies: fp16 or bf16 tensors that receive the updated parameters (None where a
     tensor has none).
@@ -45,8 +45,8 @@ class AdamW:
             raise ValueError("AdamW: betas in [0, 1) and eps >= 0 are wanted, got %r, %r" % (betas, eps))
         if state_bits not in (8, 32):
             raise ValueError("AdamW: state_bits is 32 or 8, got %r" % (state_bits,))
-        if max_norm is not None and not max_norm > 0.0:
-            raise ValueError("AdamW: max_norm must be positive, got %r" % (max_norm,))
+        if max_norm is not None and not np.float32(max_norm) > 0.0:      # as the kernel gets it
+            raise ValueError("AdamW: max_norm must be positive in fp32, got %r" % (max_norm,))
         copy_type = {c.dtype for c in copies if isinstance(c, torch.Tensor)}
         if len(copy_type) > 1 or copy_type - {torch.float16, torch.bfloat16}:
             raise ValueError("AdamW: copies of one half type are wanted, got %s" % sorted(map(str, copy_type)))
