@@ -936,8 +936,10 @@ int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy_t *opts, f
  * or in 8 bits, a half copy of the parameters) ----
  *   G = sqrt(sum g^2) over all tensors, g' = g max_norm / max(G, max_norm)            (max_norm <= 0: g' = g, G is not computed; infinite: g' = g)
  *   m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;  p -= lr (m / (1 - b1^t) / (sqrt(v / (1 - b2^t)) + eps) + decay p)
- * With clipping, a step whose G is not finite changes nothing and is counted in wd_adamw_state_t.skipped (squares are formed in fp32
- * and summed in 64 bits: an element above 1.8e19 counts as not finite).  Moment buffers start at multiples of 16 bytes.
+ * With clipping, a step whose G is not finite changes nothing and is counted in wd_adamw_state_t.skipped (the squares of eight
+ * elements are added in fp32, the rest in 64 bits: elements above 6.5e18 may count as not finite, those above 1.8e19 do).  Without
+ * clipping a gradient above 1.8e19 makes its second moment infinite with 32 bits, one above sqrt(2^128 / (1 - b2)) its block NaN with 8.
+ * Moment buffers start at multiples of 16 bytes.
  * Moments live in flat buffers, tensor k from element tensors[k].start on (a multiple of WD_ADAMW_BLOCK; buffers as long as the
  * padded sum).  bits 32: m, v float.  bits 8: m one byte of sign, 4 exponent and 3 mantissa bits, r = sqrt(v) one byte of 4 exponent
  * and 4 mantissa bits; every block of WD_ADAMW_BLOCK values has one scale byte s, the (biased) binary exponent of its largest

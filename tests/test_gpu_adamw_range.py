@@ -101,3 +101,48 @@ def test_a_max_norm_that_is_no_fp32_number_is_refused():
         with pytest.raises(ValueError, match="max_norm"):
             optim.AdamW(p, g, max_norm=bad)
     optim.AdamW(p, g, max_norm=2.0 ** -149).step()
+
+
+@pytest.mark.parametrize("grad", [torch.float32, torch.bfloat16])
+def test_largest_gradients_of_a_clipped_step(grad):
+    """The squares of eight elements are added in fp32: sqrt(2^128 / 8) = 6.5e18 is what all of them may be."""
+    from wide_deep_amd import optim
+    n = 4 * 2048 + 77
+    p = torch.zeros(n, device="cuda")
+    g = torch.full((n,), 6.4e18, device="cuda").to(grad)
+    opt = optim.AdamW([p], [g], lr=1.0, max_norm=1.0, weight_decay=0.0)
+    opt.step()
+    norm = math.sqrt(n) * float(g[0].double())
+    assert opt.skipped == 0 and opt.step_count == 1 and abs(float(opt.grad_norm) - norm) <= 10 * U * norm
+    # first step, all alike: m / sqrt(v) of the corrected moments is 1 (g' = n^-1/2 is far above eps)
+    assert bool(((p + 1.0).abs() <= 1e-5).all())
+    was = p.clone()
+    g.fill_(7e18)
+    opt.step()
+    assert opt.skipped == 1 and opt.step_count == 1 and torch.equal(p, was)
+
+
+def test_one_gradient_whose_square_is_not_finite():
+    """With clipping the step is skipped; without, 32 bits keep the parameter where it is (m / inf); 8 bits square after
+    the product with 1 - b2, 0.001 (2e19)^2 = 4e35 is in range, and keep the root."""
+    from wide_deep_amd import optim
+    for bits in (32, 8):
+        p, g = torch.zeros(256, device="cuda"), torch.full((256,), 1e-3, device="cuda")
+        g[70] = 2e19
+        opt = optim.AdamW([p], [g], lr=1.0, max_norm=1.0, weight_decay=0.0, state_bits=bits)
+        opt.step()
+        assert opt.skipped == 1 and bool((p == 0).all())
+        opt = optim.AdamW([p], [g], lr=1.0, weight_decay=0.0, state_bits=bits)
+        opt.step()
+        others = torch.arange(256, device="cuda") != 70
+        assert bool(((p[others] + 1).abs() < 1e-3).all())
+        if bits == 32:
+            assert float(p[70]) == 0.0 and float(opt.v[70]) == math.inf
+        else:
+            m, r = opt.moments(torch.float32)
+            assert abs(float(p[70]) + 1) < 1e-3 and bool(m.isfinite().all()) and bool(r.isfinite().all())
+            assert abs(float(r[70]) / (math.sqrt(0.001) * 2e19) - 1) <= 2.0 ** -4         # a step of 4 bits
+            g[70] = 1e21                                                                  # 0.001 (1e21)^2 = 1e39 is not
+            opt.step()
+            m, r = opt.moments()
+            assert bool(p[70].isnan()) and bool(r[64:128].isnan().all()) and bool(r[:64].isfinite().all()) and bool(r[128:].isfinite().all())

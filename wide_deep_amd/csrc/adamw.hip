@@ -177,7 +177,7 @@ k_grad_square(const wd_adamw_tensor_t *__restrict__ tensors, const int32_t *__re
     for (int c = 0; c < C; ++c) y[c] = chunk_of<GT>(tensors, chunks, min(c0 + (int64_t)(C + c) * gridDim.x, last));
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      float s = 0.f;      // 8 squares in fp32, then 64 bits
+      float s = 0.f;      // 8 squares in fp32 (finite up to sqrt(2^128 / 8) = 6.5e18 each), then 64 bits
 #pragma unroll
       for (int u = 0; u < N; ++u)
 #pragma unroll

@@ -22,7 +22,7 @@ _OPTS = struct.Struct("=QQqQQQQQQQQddfffIiiii")     # wd_adamw_t
 class AdamW:
     """params, grads: lists of contiguous tensors on one GPU, fp32 and fp32 / fp16 / bf16 (one type for all gradients), bound for good.
     weight_decay: one number or one per tensor.  max_norm: clip by the global norm of all gradients (math.inf: tell it and clip nothing); a step whose norm is not finite
-    (an element above 1.8e19, too: its square is formed in fp32) changes nothing and is counted in `skipped`.  state_bits: 32, or 8 (m and the root r of the second moment, one byte each; rounding by
+    (elements above 6.5e18 may do that: the squares of eight are added in fp32) changes nothing and is counted in `skipped`.  state_bits: 32, or 8 (m and the root r of the second moment, one byte each; rounding by
     a hash of index, step and `seed`, so runs repeat; elements whose root is below 2^-18 of the largest of their 64 take smaller steps than with 32).  copies: fp16 or bf16 tensors that receive the updated parameters (None where a
     tensor has none).
 
