@@ -18,8 +18,8 @@ import torch
 
 from . import capi, hipgraph
 from .capi import call, ptr
-from .plan import (BN_EPS, FeaturePlan, ModelSpec, OPT_SLOT_ODD, adam_pow_names, bucket_geometry, ftrl_l2_shrinkage, ftrl_lr_power, opt_params,
-                   opt_slot_init, opt_slot_names, rmsprop_centered, small_table_slots)
+from .plan import (ADAMW_STEPS, BN_EPS, FeaturePlan, ModelSpec, OPT_SLOT_ODD, adam_pow_names, bucket_geometry, ftrl_l2_shrinkage, ftrl_lr_power, opt_params,
+                   opt_slot_init, opt_slot_names, rmsprop_centered, small_table_slots, steps_of_powers)
 
 
 class DeviceBatch:
@@ -476,7 +476,7 @@ class WideDeepEngine:
         return optim.AdamW([p for p, _ in params], [g for g, _ in self._dense_tensors(self.G)], lr=opt[1], betas=(opt[2], opt[3]), eps=opt[4],
                            weight_decay=[float(opt[5]) if kernel else 0.0 for _, kernel in params], max_norm=opt[6])
 
-    def _sync_adamw(self, load):
+    def _sync_adamw(self, load, state=None):
         """Moments of the dense parameters: optimizer -> Pa / Pacc (what export_state reads), or back with the step count of an import."""
         if not self.spec.has_deep or self.adamw is None:
             return
@@ -484,10 +484,10 @@ class WideDeepEngine:
             for start, (t, _) in zip(self.adamw.starts, self._dense_tensors(buf)):
                 part = flat[start: start + t.numel()]
                 part.copy_(t) if load else t.copy_(part)
-        if load:
-            # beta2^(t + 1) is the checkpoint's non-slot variable; at 0 (below fp32) the corrections are 1 whatever t
-            power, beta = float(self.pow["dnn"][1]), self.adamw.betas[1]
-            self.adamw.set_step(max(0, round(math.log(power) / math.log(beta)) - 1) if 0.0 < power < 1.0 and beta > 0.0 else 10 ** 6)
+        if load and ADAMW_STEPS in state:
+            self.adamw.set_step(*(int(x) for x in state[ADAMW_STEPS].reshape(-1)))
+        elif load and self.pow_names["dnn"][0] in state:      # a file of the Adam that shares its names, or one from before the count was kept
+            self.adamw.set_step(steps_of_powers(self.adamw.betas, [float(x) for x in self.pow["dnn"]]))
 
     def _opt_dense(self, st):
         """Any optimizer but the default Adagrad on the dense parameters of the dnn scope, gradients in G."""
@@ -1594,6 +1594,8 @@ class WideDeepEngine:
                 out["linear/linear_model/bias_weights" + suf] = (1,)
         for scope, names in self.pow_names.items():
             out[names[0]], out[names[1]] = (), ()
+        if self.adamw is not None:
+            out[ADAMW_STEPS] = (2,)
         out["global_step"] = ()
         return out
 
@@ -1645,6 +1647,8 @@ class WideDeepEngine:
         for scope, names in self.pow_names.items():
             pw = self.pow[scope].cpu()
             out[names[0]], out[names[1]] = pw[0].clone(), pw[1].clone()
+        if self.adamw is not None:
+            out[ADAMW_STEPS] = torch.tensor([self.adamw.step_count, self.adamw.skipped], dtype=torch.int64)
         out["global_step"] = torch.tensor(self.global_step, dtype=torch.int64)
         return out
 
@@ -1696,7 +1700,7 @@ class WideDeepEngine:
             if names[0] in state:
                 self.pow[scope][0] = float(state[names[0]])
                 self.pow[scope][1] = float(state[names[1]])
-        self._sync_adamw(load=True)
+        self._sync_adamw(True, state)
         self._primed = None
         if "global_step" in state:
             self.global_step = int(state["global_step"])

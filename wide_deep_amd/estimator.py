@@ -23,6 +23,7 @@ import torch
 
 from .engine import DeviceBatch, WideDeepEngine
 from .features import Featurizer
+from .plan import ADAMW_STEPS
 
 
 class _GraphStep(object):
@@ -258,7 +259,8 @@ class WideAndDeepClassifier(object):
                 want[k] = shape
         else:
             want = self._engine.state_shapes()
-        skip = lambda k: k == "global_step" or k.endswith("/moving_mean") or k.endswith("/moving_variance")
+        # (ADAMW_STEPS: the beta powers tell it where a file has none)
+        skip = lambda k: k in ("global_step", ADAMW_STEPS) or k.endswith("/moving_mean") or k.endswith("/moving_variance")
         missing = sorted(k for k in want if k not in state and not skip(k))
         if missing:
             raise ValueError("%s does not hold %d of the variables this model restores by name (first: %s); variables of the "

@@ -118,9 +118,11 @@ class AdamW:
             rate, dev_rate = 0.0, lr.data_ptr()
         self._call("wd_adamw_step", _OPTS.pack(*self._head, dev_rate, *self.betas, rate, self.eps, self.max_norm or 0.0, self.seed, *self._types))
 
-    def set_step(self, step):
-        """The number of steps done so far (a restored optimizer); clears `skipped`."""
+    def set_step(self, step, skipped=0):
+        """The number of steps done and skipped so far (a restored optimizer)."""
         self._call("wd_adamw_set_step", self._state.data_ptr(), self._tickets.data_ptr(), int(step), *self.betas)
+        if skipped:
+            self._state[2].fill_(int(skipped))
 
     @property
     def step_count(self):

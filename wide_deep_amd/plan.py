@@ -576,6 +576,35 @@ def adam_pow_names(dnn_opt, lin_opt, has_deep, has_wide):
     return out
 
 
+#: AdamW's steps done and steps skipped, int64 [2]: the beta powers above count the tables' steps, which skip none
+ADAMW_STEPS = "dnn/AdamW/steps"
+
+
+def steps_of_powers(betas, powers):
+    """Steps done, from the beta powers of a checkpoint without ADAMW_STEPS.  They are beta^(steps + 1) as products of fp32, each rounded, so
+    the product is repeated until it meets the power; the larger beta's, which stays in fp32 longer.  A power that has left the normal
+    numbers: the step at which it does, where 1 - beta^t is 1 already."""
+    beta, power = max(zip(betas, powers))
+    b = np.float32(beta)
+    if not 0.0 < b < 1.0 or power >= b:
+        return 0
+    last = int(math.ceil(126.0 / -math.log2(b)))
+    if power < 2.0 ** -126:
+        return last
+    done, product = 0, np.float32(1.0)
+    while done <= last:
+        part = np.full(1 << 16, b, dtype=np.float32)
+        part[0] *= product
+        part = np.multiply.accumulate(part)
+        product = part[-1]
+        if product <= power:
+            k = int(np.searchsorted(-part, -power))           # the first one that is not above it, or the one in front
+            before = part[k - 1] if k else np.float32(math.inf)
+            return done + k - (1 if before - power < power - part[k] else 0)
+        done += len(part)
+    return last
+
+
 def bucket_geometry(vocab_sizes, occ_per_slot, nb_max, target=64.0):
     """Row-range buckets of the fused sparse backward (wd_sparse_bucketize): slot s is cut into ceil(V_s / 2^shift_s)
     buckets of 2^shift_s consecutive rows, sized for ~`target` occurrences per bucket when ids are uniform.  A slot
