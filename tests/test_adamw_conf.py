@@ -1,4 +1,4 @@
-"""CPU: AdamW around the engine -- the step count of a checkpoint."""
+"""CPU: AdamW around the engine -- the step count of a checkpoint, and what is told of skipped steps."""
 
 import numpy as np
 import pytest
@@ -21,3 +21,26 @@ def test_steps_from_the_powers_of_a_checkpoint(betas):
         else:
             assert top ** got < 2.0 ** -100
     assert steps_of_powers(betas, list(betas)) == 0 and steps_of_powers((0.0, 0.0), (0.0, 0.0)) == 0
+
+
+def test_skipped_steps_are_told(capsys):
+    """What a training run skipped is told once, what a checkpoint brought along is not."""
+    from types import SimpleNamespace
+    from wide_deep_amd.estimator import WideAndDeepClassifier
+    opt = SimpleNamespace(max_norm=1.0, skipped=2)
+    est = WideAndDeepClassifier(None, engine=SimpleNamespace(adamw=opt))
+
+    def told():
+        est._tell_skipped()
+        return capsys.readouterr().out
+
+    assert told() == ""
+    opt.skipped = 5
+    assert told().startswith("WARNING: 3 train steps") and told() == ""
+    opt.skipped = 6
+    assert told().startswith("WARNING: 1 train steps")
+    opt.max_norm, opt.skipped = None, 9
+    assert told() == ""
+    for engine in (SimpleNamespace(adamw=None), SimpleNamespace()):
+        est = WideAndDeepClassifier(None, engine=engine)
+        assert told() == ""

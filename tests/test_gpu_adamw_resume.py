@@ -84,3 +84,16 @@ def test_a_state_without_counters_leaves_the_count_alone():
     state = {k: v for k, v in a.export_state().items() if k not in ("dnn/AdamW/steps", "beta1_power", "beta2_power", "global_step")}
     a.import_state(state)
     assert a.adamw.step_count == 10
+
+
+def test_max_norm_guards_the_dense_parameters_alone():
+    """Inputs of 1e30: the kernels' gradients have no finite norm, the tables' gradients are ordinary.  The towers stay, the tables step."""
+    a = _engine(4)
+    a.train_step(_batch(a, 1))
+    bt = _batch(a, 2)
+    bt.dense[:, 1] = 1e30                        # every example: one at least is answered wrongly through a unit that is on
+    P, emb = a.P.clone(), a.emb.clone()
+    a.train_step(bt)
+    torch.cuda.synchronize()
+    assert a.adamw.skipped == 1 and a.adamw.step_count == 1 and not math.isfinite(float(a.adamw.grad_norm))
+    assert torch.equal(a.P, P) and not torch.equal(a.emb, emb) and bool(a.emb.isfinite().all())

@@ -469,7 +469,9 @@ class WideDeepEngine:
 
     def _make_adamw(self):
         """dnn_opt ("AdamW", lr, beta1, beta2, epsilon, weight_decay, max_norm): one step over the tensors of P, decay on the kernels.
-        Its moments stand in buffers of its own; Pa / Pacc hold them for checkpoints (_sync_adamw)."""
+        Its moments stand in buffers of its own; Pa / Pacc hold them for checkpoints (_sync_adamw).
+        max_norm guards the dense parameters alone: a step whose norm is not finite leaves them as they are (`adamw.skipped` counts it), but
+        the tables, updated beside the towers before that norm is known, take its gradients, as with every other optimizer."""
         from . import optim
         opt = self.spec.dnn_opt
         params = self._dense_tensors(self.P)

@@ -92,6 +92,7 @@ class WideAndDeepClassifier(object):
         self._graph_steps = {}        # batch size -> _GraphStep (captured featurizer + train step)
         self._warm = {}               # batch size -> the first RawBatches of that size (eager steps; they size the fixed stage)
         self._nnz_seen = 0
+        self._skipped_told = None     # steps that AdamW had skipped when it was last told
 
     # ---- engine life cycle --------------------------------------------------------------------------
     def _ensure_engine(self, first_batch):
@@ -137,6 +138,17 @@ class WideAndDeepClassifier(object):
         """Row-sharded engine: a peer segment that overflowed dropped occurrences (include/wd_hip.h) -- never silently."""
         if self._engine is not None and hasattr(self._engine, "check_overflow"):
             self._engine.check_overflow()
+
+    def _tell_skipped(self):
+        """AdamW(max_norm=...): a step whose gradient norm was not finite left the dense parameters as they were, but the tables took it."""
+        opt = getattr(self._engine, "adamw", None)
+        if opt is None or opt.max_norm is None:
+            return
+        n, told = opt.skipped, self._skipped_told
+        self._skipped_told = n
+        if told is not None and n > told and self._rank() == 0:
+            print("WARNING: %d train steps had a gradient norm that is not finite: AdamW left the dense parameters out of them, the embedding and "
+                  "linear tables took their gradients" % (n - told))
 
     def _save_due(self, n, t_save, save_secs):
         """Timed checkpoints.  One process: the local clock.  Several ranks: saving is a collective, so rank 0's clock
@@ -337,6 +349,8 @@ class WideAndDeepClassifier(object):
                 bt = self._device_batch(raw)
             if n == 0:
                 self._restore()
+                self._skipped_told = None
+                self._tell_skipped()
                 t0 = time.time()       # examples/sec of the loop itself: checkpoint restore / save are reported apart
                 if max_steps is not None and self._engine.global_step >= max_steps:
                     break
@@ -368,6 +382,7 @@ class WideAndDeepClassifier(object):
                 dt = time.time() - t0
                 print("INFO: step %d (global_step %d): loss = %.6f, %.1f examples/sec" % (
                     n, self._engine.global_step, float(loss), seen / max(dt, 1e-9)))
+                self._tell_skipped()
             if n % self._CHECK_EVERY == 0:
                 self._check_overflow()
             if self._save_due(n, t_save, save_secs):
@@ -381,6 +396,7 @@ class WideAndDeepClassifier(object):
         if n:
             torch.cuda.synchronize()
             self._check_overflow()
+            self._tell_skipped()
             for g in self._graph_steps.values():
                 if g:
                     g.check()

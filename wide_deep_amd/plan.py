@@ -120,7 +120,8 @@ class ModelSpec:
     # optimizer tuples (build_estimator.opt_tuple): ("SGD", lr) ("Adagrad", lr, init_accum) ("Ftrl", lr, l1, l2, init_accum)
     # ("RMSProp", lr, decay, momentum, epsilon) ("Adam", lr, beta1, beta2, epsilon)
     # dnn_opt also ("AdamW", lr, beta1, beta2, epsilon, weight_decay, max_norm or None): optim.AdamW on the tower's parameters
-    # (weight decay on its kernels, clipping by the norm of all of them), Adam on the embedding tables
+    # (weight decay on its kernels, clipping by the norm of all of them), Adam on the embedding tables; a step whose norm is not finite
+    # is left out by the tower's parameters, not by the tables
     dnn_opt: tuple = ("Adagrad", 0.05, 0.1)
     lin_opt: tuple = ("Ftrl", 0.1, 0.5, 1.0, 0.1)
     use_weight_column: bool = False
