@@ -1,9 +1,15 @@
-"""CPU: AdamW around the engine -- the step count of a checkpoint, and what is told of skipped steps."""
+"""CPU: AdamW around the engine -- `dnn_optimizer: AdamW` in model.yaml (by name, as a constructor, its rate's decay, what is refused) and the
+step count of a checkpoint."""
+import shutil
 
 import numpy as np
 import pytest
+import yaml
 
+from wide_deep_amd import build_estimator as BE
+from wide_deep_amd.build_estimator import opt_tuple, parse_optimizer
 from wide_deep_amd.plan import steps_of_powers
+from wide_deep_amd.read_conf import Config, conf_dir
 
 
 @pytest.mark.parametrize("betas", [(0.9, 0.999), (0.9, 0.99), (0.9, 0.9999), (0.9, 0.99999), (0.99, 0.5), (0.9, 0.0), (0.0, 0.9)])
@@ -44,3 +50,23 @@ def test_skipped_steps_are_told(capsys):
     for engine in (SimpleNamespace(adamw=None), SimpleNamespace()):
         est = WideAndDeepClassifier(None, engine=engine)
         assert told() == ""
+
+
+def test_the_rate_of_an_adamw_given_by_name_decays(tmp_path):
+    """lr_decay applies to optimizers given by name: AdamW as any other; a constructor keeps its own rate."""
+    base = tmp_path / "conf"
+    shutil.copytree(conf_dir(), base)
+    tr = yaml.safe_load(open(base / "train.yaml"))
+    tr["train"]["lr_decay"] = True
+    yaml.safe_dump(tr, open(base / "train.yaml", "w"))
+    m = yaml.safe_load(open(base / "model.yaml"))
+    got = {}
+    for name in ("Adam", "AdamW", " AdamW ", "AdamW(0.002)"):
+        m["dnn_optimizer"] = name
+        yaml.safe_dump(m, open(base / "model.yaml", "w"))
+        conf = Config(base_dir=str(base))
+        spec = BE.build_model_spec(conf, "wide_deep")
+        got[name] = spec.lr_decay
+        assert spec.dnn_opt[0] == name.strip().split("(")[0]
+    steps = conf.train["num_examples"] / conf.train["batch_size"]
+    assert got["Adam"] == got["AdamW"] == got[" AdamW "] == {"dnn": (0.8, steps)} and got["AdamW(0.002)"] is None

@@ -36,6 +36,12 @@ def _unsupported(opt):
     return ValueError("Unsupported optimizer option: `%s`. Supported names are: %s or an `Optimizer` instance." % (opt, _OPT_NAMES))
 
 
+def given_by_name(opt):
+    """Whether an optimizer option is one of the names, which take the model_fn's learning rate; AdamW is not the reference's
+    (plan.ModelSpec.dnn_opt)."""
+    return str(opt).strip() in tuple(_OPT_NAMES) + ("AdamW",)
+
+
 def parse_optimizer(opt, default_lr):
     """'Adagrad' | 'tf.train.FtrlOptimizer(learning_rate=0.1, l1_regularization_strength=0.5, ...)' -> (name, kwargs).
     The reference eval()s constructor strings (python/lib/utils/model_util.py:62-105); here the expression is parsed
@@ -44,7 +50,7 @@ def parse_optimizer(opt, default_lr):
     if not isinstance(opt, str):
         raise ValueError("optimizer must be a string, got %r" % (opt,))
     text = opt.strip()
-    if text in _OPT_NAMES or text == "AdamW":           # AdamW: not the reference's (plan.ModelSpec.dnn_opt)
+    if given_by_name(text):
         if default_lr is None:
             raise ValueError("learning_rate must be specified when opt is supported string.")
         return text, {"learning_rate": default_lr}
@@ -177,7 +183,7 @@ def build_model_spec(conf=None, model_type=None):
         lr_decay = {}
         for scope, key, rk in (("dnn", "dnn_optimizer", "dnn_decay_rate"), ("linear", "linear_optimizer", "linear_decay_rate")):
             rate = model.get(rk) or 1
-            if str(model[key]).strip() in _OPT_NAMES and float(rate) != 1.0:
+            if given_by_name(model[key]) and float(rate) != 1.0:
                 lr_decay[scope] = (float(rate), steps)
     # weight column is switched on when EITHER weight is set (build_estimator.py:43-46) ...
     use_w = train["pos_sample_loss_weight"] is not None or train["neg_sample_loss_weight"] is not None
