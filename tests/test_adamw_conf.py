@@ -1,5 +1,6 @@
 """CPU: AdamW around the engine -- `dnn_optimizer: AdamW` in model.yaml (by name, as a constructor, its rate's decay, what is refused) and the
 step count of a checkpoint."""
+import math
 import shutil
 
 import numpy as np
@@ -70,3 +71,22 @@ def test_the_rate_of_an_adamw_given_by_name_decays(tmp_path):
         assert spec.dnn_opt[0] == name.strip().split("(")[0]
     steps = conf.train["num_examples"] / conf.train["batch_size"]
     assert got["Adam"] == got["AdamW"] == got[" AdamW "] == {"dnn": (0.8, steps)} and got["AdamW(0.002)"] is None
+
+
+@pytest.mark.parametrize("text,message", [
+    ("AdamW(lr=0.0003)", "lr"), ("AdamW(0.001, betas=(0.9, 0.95))", "betas"), ("AdamW(0.001, eps=1e-6)", "eps"), ("AdamW(0.001, state_bits=8)", "state_bits"),
+    ("AdamW(0.001, 0.9, 0.95)", "by name"), ("AdamW(0.001, learning_rate=0.002)", "learning_rate"), ("AdamW(**{'beta1': 0.8})", "by name"),
+    ("AdamW(0.001, max_norm=0)", "max_norm"), ("AdamW(0.001, max_norm=-1.0)", "max_norm"), ("AdamW(0.001, weight_decay=-1)", "weight_decay"),
+    ("AdamW(0.001, beta1=1.0)", "beta1"), ("AdamW(0.001, beta2=-0.1)", "beta2"), ("AdamW(0.001, epsilon=-1e-8)", "epsilon")])
+def test_arguments_that_would_be_dropped_or_cannot_be_are_refused(text, message):
+    with pytest.raises(ValueError, match=message):
+        opt_tuple(*parse_optimizer(text, 0.05))
+
+
+def test_arguments_that_are_taken():
+    assert opt_tuple(*parse_optimizer("AdamW()", 0.05)) == ("AdamW", 0.001, 0.9, 0.999, 1e-8, 0.01, None)
+    assert opt_tuple(*parse_optimizer("optim.AdamW(learning_rate=0.01, beta1=0.8, beta2=0.9, epsilon=1e-6, weight_decay=0, max_norm=None)", 0.05)) == (
+        "AdamW", 0.01, 0.8, 0.9, 1e-6, 0.0, None)
+    assert opt_tuple(*parse_optimizer("AdamW(0.01, max_norm=1e999)", 0.05))[6] == math.inf
+    # the reference's constructors stay as they were
+    assert opt_tuple(*parse_optimizer("tf.train.AdamOptimizer(0.01, name='x')", 0.05)) == ("Adam", 0.01, 0.9, 0.999, 1e-8)

@@ -67,6 +67,8 @@ def parse_optimizer(opt, default_lr):
     if cls != "AdamW" and (cls not in _OPT_ALIASES or not cls.endswith("Optimizer")):
         # tf.train has no such class (AttributeError in the reference) -- or it has, and this engine does not build it
         raise _unsupported(opt)
+    if cls == "AdamW":
+        _check_adamw_call(node, text)
     kwargs = {}
     if node.args:
         kwargs["learning_rate"] = ast.literal_eval(node.args[0])
@@ -76,6 +78,19 @@ def parse_optimizer(opt, default_lr):
     name = _OPT_ALIASES.get(cls, cls)
     kwargs.setdefault("learning_rate", 0.001 if name in ("Adam", "AdamW") else default_lr)
     return name, kwargs
+
+
+_ADAMW_ARGS = ("learning_rate", "beta1", "beta2", "epsilon", "weight_decay", "max_norm")
+
+
+def _check_adamw_call(node, text):
+    """AdamW(learning_rate, beta1=, ...): an argument that would not be taken is refused, those of optim.AdamW under other names too."""
+    names = ["learning_rate"] * len(node.args[:1]) + [kw.arg for kw in node.keywords]
+    if len(node.args) > 1 or None in names:
+        raise ValueError("AdamW takes the learning rate first and everything else by name (%s): got `%s`" % (", ".join(_ADAMW_ARGS), text))
+    for n in names:
+        if n not in _ADAMW_ARGS or names.count(n) > 1:
+            raise ValueError("AdamW: `%s` is %s; it takes %s: got `%s`" % (n, "given twice" if n in _ADAMW_ARGS else "none of its arguments", ", ".join(_ADAMW_ARGS), text))
 
 
 def opt_tuple(name, kw):
@@ -113,8 +128,14 @@ def opt_tuple(name, kw):
         return ("Adam", lr, float(kw.get("beta1", 0.9)), float(kw.get("beta2", 0.999)), float(kw.get("epsilon", 1e-8)))
     if name == "AdamW":
         max_norm = kw.get("max_norm")
-        return ("AdamW", lr, float(kw.get("beta1", 0.9)), float(kw.get("beta2", 0.999)), float(kw.get("epsilon", 1e-8)),
-                float(kw.get("weight_decay", 0.01)), None if max_norm is None else float(max_norm))
+        opt = ("AdamW", lr, float(kw.get("beta1", 0.9)), float(kw.get("beta2", 0.999)), float(kw.get("epsilon", 1e-8)),
+               float(kw.get("weight_decay", 0.01)), None if max_norm is None else float(max_norm))
+        for what, value, ok in (("beta1 in [0, 1)", opt[2], 0.0 <= opt[2] < 1.0), ("beta2 in [0, 1)", opt[3], 0.0 <= opt[3] < 1.0),
+                                ("epsilon >= 0", opt[4], opt[4] >= 0.0), ("weight_decay >= 0", opt[5], opt[5] >= 0.0),
+                                ("max_norm > 0", opt[6], opt[6] is None or opt[6] > 0.0)):
+            if not ok:
+                raise ValueError("AdamW: %s is wanted, got %r" % (what, value))
+        return opt
     raise ValueError("Unsupported optimizer: %s" % name)
 
 
