@@ -1159,10 +1159,8 @@ extern "C" int wd_bucket_sort_ragged(const int32_t *bucket_start, uint64_t *pair
   g.bag_bits = 1;
   while (g.bag_bits < 32 && ((int64_t)1 << g.bag_bits) < batch * S) ++g.bag_bits;
   hipStream_t st = wd::as_stream(stream);
-  if (hipMemsetAsync(long_list, 0, 8, st) != hipSuccess) {      // the two counters wd_bucket_onehot zeroes on the one-id-per-bag path
-    wd::set_error("wd_bucket_sort_ragged: hipMemsetAsync failed");
-    return WD_ERR_LAUNCH;
-  }
+  // the two counters wd_bucket_onehot zeroes on the one-id-per-bag path
+  if (const int rc = wd_fill_f32(reinterpret_cast<float *>(long_list), 0.f, 2, stream)) return rc;
   static const int wave_sort = getenv("WD_SORT_WAVE") ? atoi(getenv("WD_SORT_WAVE")) : 1;
   if (wave_sort) hipLaunchKernelGGL(k_bucket_sort_wave, dim3((unsigned)wd::ceil_div(nbuckets, 4)), dim3(256), 0, st, g);
   else hipLaunchKernelGGL(k_bucket_sort_small, dim3((unsigned)nbuckets), dim3(256), 0, st, g);

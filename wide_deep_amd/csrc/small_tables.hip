@@ -490,11 +490,7 @@ extern "C" int wd_small_tables_grad(const wd_slot_t *slots, int32_t S, const int
   a.emb_w = a.emb_acc = a.wide_w = nullptr;
   hipStream_t st = wd::as_stream(stream);
   if (batch <= 0) {        // a rank without examples still takes part in the all-reduce: zeros
-    if (hipMemsetAsync(gsum, 0, sizeof(float) * (size_t)nsmall * max_rows * (max_dim + 2), st) != hipSuccess) {
-      wd::set_error("wd_small_tables_grad: hipMemsetAsync failed");
-      return WD_ERR_LAUNCH;
-    }
-    return wd::check_launch("wd_small_tables_grad");
+    return wd_fill_f32(gsum, 0.f, (int64_t)nsmall * max_rows * (max_dim + 2), stream);
   }
   hipLaunchKernelGGL(k_small_bwd, dim3((unsigned)a.nslice, (unsigned)nsmall), dim3(256), lds, st, a);
   hipLaunchKernelGGL(k_small_reduce, dim3((unsigned)wd::ceil_div((int64_t)max_rows * (max_dim + 2) * SM_AP, (int64_t)256), (unsigned)nsmall),

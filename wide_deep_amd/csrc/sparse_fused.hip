@@ -1012,7 +1012,7 @@ k_opt_dense(float *__restrict__ w, float *__restrict__ sa, float *__restrict__ s
 
 // Adam moves EVERY row of a sparsely updated variable (AdamOptimizer._apply_sparse_shared assigns m*beta1, v*beta2 and
 // the var update over the whole variable): rows without a gradient this step, marked 0 in `touched`, get g = 0 here.
-// One thread per (row, 4-float chunk) of a slot / per wide line; the bitmap is cleared by wd_adam_untouched's memset.
+// One thread per (row, 4-float chunk) of a slot / per wide line; the bitmap is cleared by the fill behind it.
 __global__ void __launch_bounds__(256)
 k_adam_untouched_emb(float *__restrict__ emb, float *__restrict__ m, float *__restrict__ v,
                      const wd_slot_t *__restrict__ slots, const uint32_t *__restrict__ touched, OptK o,
@@ -1088,10 +1088,7 @@ extern "C" int wd_adam_untouched(float *emb, float *emb_m, float *emb_v, float *
     hipLaunchKernelGGL(k_adam_untouched_wide, dim3(gx, (unsigned)S), dim3(256), 0, st, wide, slots, touched,
                        to_optk(wide_opt), wide_opt->pow);
   }
-  if (hipMemsetAsync(touched, 0, (size_t)((total_rows + 31) / 32) * 4, st) != hipSuccess) {
-    wd::set_error("wd_adam_untouched: hipMemsetAsync failed");
-    return WD_ERR_LAUNCH;
-  }
+  if (const int rc = wd_fill_f32(reinterpret_cast<float *>(touched), 0.f, (total_rows + 31) / 32, stream)) return rc;
   return wd::check_launch("wd_adam_untouched");
 }
 
