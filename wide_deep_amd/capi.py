@@ -285,14 +285,14 @@ class WdError(RuntimeError):
 
 
 def source_stamp():
-    """sha256 over csrc/*.hip, csrc/*.h and include/wd_hip.h in name order -- what csrc/build.sh embeds as wd_build_stamp().
+    """sha256 over csrc/*.hip, csrc/*.h, csrc/build.sh and include/wd_hip.h in name order -- what csrc/build.sh embeds as wd_build_stamp().
     None when the sources are not there (an installed library without its tree)."""
     import glob
     import hashlib
     csrc = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
     names = sorted([os.path.basename(f) for f in glob.glob(os.path.join(csrc, "*.hip")) + glob.glob(os.path.join(csrc, "*.h"))]
-                   + ["../../include/wd_hip.h"])
-    if len(names) < 3:
+                   + ["build.sh", "../../include/wd_hip.h"])
+    if len(names) < 4:
         return None
     h = hashlib.sha256()
     try:

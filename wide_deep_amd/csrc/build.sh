@@ -6,18 +6,24 @@ OUT="$HERE/../_lib"
 mkdir -p "$OUT" "$HERE/_obj"
 # packed fp32 instructions (v_pk_add / mul / fma_f32) are kept out: some of their forms have given wrong results on this hardware
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops"
+# an object is made again when its source, any header or this script (its flags) is newer, and always with WD_REBUILD set
 pids=""
 for f in common hash embag sparse_update sparse_fused small_tables onehot_path dist_exchange mlp mlp_half mlp_chain mlp_chain8 policy_loss adamw; do
-  if [ ! -f "$HERE/_obj/$f.o" ] || [ "$HERE/$f.hip" -nt "$HERE/_obj/$f.o" ] || [ "$HERE/common.h" -nt "$HERE/_obj/$f.o" ] || [ "$HERE/mlp_chain.h" -nt "$HERE/_obj/$f.o" ] \
-     || [ "$HERE/../../include/wd_hip.h" -nt "$HERE/_obj/$f.o" ]; then
-    hipcc $FLAGS -c "$HERE/$f.hip" -o "$HERE/_obj/$f.o" &
+  obj="$HERE/_obj/$f.o"
+  stale="$WD_REBUILD"
+  for dep in "$HERE/$f.hip" "$HERE"/*.h "$HERE/../../include/wd_hip.h" "$HERE/build.sh"; do
+    if [ ! -f "$obj" ] || [ "$dep" -nt "$obj" ]; then stale=1; fi
+  done
+  if [ -n "$stale" ]; then
+    rm -f "$obj"
+    hipcc $FLAGS -c "$HERE/$f.hip" -o "$obj" &
     pids="$pids $!"
   fi
 done
 for p in $pids; do wait $p; done
-# source stamp: sha256 over the sources this library is built from (sorted by name; capi.load() recomputes it and refuses a
-# library that was built from other sources -- the prebuilt .so travels to the GPU box, a stale one would otherwise load silently)
-STAMP=$(cd "$HERE" && cat $(ls *.hip *.h ../../include/wd_hip.h | LC_ALL=C sort) | sha256sum | cut -c1-64)
+# source stamp: sha256 over the sources this library is built from and this script's flags (sorted by name; capi.load() recomputes it and
+# refuses a library that was built from others -- a prebuilt .so travels with the tree, a stale one would otherwise load silently)
+STAMP=$(cd "$HERE" && cat $(ls *.hip *.h build.sh ../../include/wd_hip.h | LC_ALL=C sort) | sha256sum | cut -c1-64)
 printf 'extern "C" const char *wd_build_stamp(void) { return "%s"; }\n' "$STAMP" > "$HERE/_obj/build_stamp.cpp"
 g++ -O1 -fPIC -c "$HERE/_obj/build_stamp.cpp" -o "$HERE/_obj/build_stamp.o"
 hipcc --offload-arch=gfx950 -shared -fPIC "$HERE"/_obj/build_stamp.o "$HERE"/_obj/common.o "$HERE"/_obj/hash.o "$HERE"/_obj/embag.o \
