@@ -868,7 +868,8 @@ int wd_small_tables_apply(float *emb, float *emb_accum, float *wide_wzn, const w
  * hold NaN --, its log-probability is 0 and its gradient 0.  Sequences are a CSR over the rows: sequence n = rows [seq_offs[n],
  * seq_offs[n + 1]), ascending; rows in front of the first and behind the last sequence belong to nobody: token_logp there is 0, a
  * gradient buffer is left as it was (zero_tail != 0: zeroed).  An item with logit -inf has probability 0.  Rows may start at any
- * multiple of the element size.  dlogits may be the logits' own buffer; no other output may share memory with an input.  ws:
+ * multiple of the element size.  dlogits may be the logits' own buffer (same rows, same stride; any other overlap of the two is refused);
+ * no other output may share memory with an input.  ws:
  * wd_policy_workspace_floats(rows) floats, 8-byte aligned, for one call at a time (negative: the arguments are refused).  At most
  * 2^30 rows and items, 2^29 sequences.  All launches go to `stream`; nothing is read back. */
 #define WD_T_F32 0

@@ -127,3 +127,24 @@ def test_pairs_of_weight_zero_add_nothing(rows, vocab, dtype, kind):
     want = float((r.pair_loss[1:].double() * 0.5).sum())
     assert abs(float(r.loss) - want) <= 2.0 ** -23 * want      # pair_loss and loss round once each
     assert bool((r.dlogits[a:c] == 0).all()) and bool(r.dlogits.isfinite().all()) and bool((r.dlogits[c:] != 0).any())
+
+
+def test_gradients_beside_the_logits_rows():
+    """Logits and gradient as halves of one buffer's rows are apart; places that share memory with the logits without being theirs are refused."""
+    from wide_deep_amd import capi, policy
+    for rows, vocab in ((8, 40), (300, 1001), (12, 70001)):
+        g = torch.Generator("cuda").manual_seed(rows)
+        both = torch.randn(rows, 2 * vocab, device="cuda", generator=g)
+        z, place = both[:, :vocab], both[:, vocab:]
+        t = torch.randint(0, vocab, (rows,), device="cuda", generator=g, dtype=torch.int32)
+        offs = torch.tensor([0, rows // 4, rows // 2, rows - 1, rows], device="cuda", dtype=torch.int32)
+        adv, old = torch.randn(4, device="cuda", generator=g), policy.sequence_logp(z, t, offs).token_logp - 0.1
+        for call in (lambda g: policy.preference_loss(z, t, offs, dlogits=g), lambda g: policy.policy_loss(z, t, offs, old, adv, per_row=False, dlogits=g)):
+            was = z.clone()
+            want = call(True).dlogits
+            got = call(place)
+            assert got.dlogits is place and torch.equal(place, want) and torch.equal(z, was)
+            for bad in (both[:, 1: vocab + 1], both[:, vocab - 1: 2 * vocab - 1]):
+                with pytest.raises(capi.WdError, match="shares memory"):
+                    call(bad)
+            assert torch.equal(z, was)

@@ -1116,6 +1116,32 @@ int check_rows(const char *who, const wd_seq_rows_t *q) {
   return WD_OK;
 }
 
+// whether a row of one of two matrices of `rows` rows of `w` bytes, `s` and `t` bytes apart, meets a row of the other without their being the
+// same matrix.  Rows of either between the other's (s == t, a wider buffer of both) are apart.
+bool meet(const void *a, int64_t s, const void *b, int64_t t, int64_t rows, int64_t w) {
+  int64_t d = (int64_t)((uintptr_t)b - (uintptr_t)a);
+  if (rows < 1 || (d == 0 && (s == t || rows == 1)) || d >= (rows - 1) * s + w || -d >= (rows - 1) * t + w) return false;
+  if (s == t) {
+    const int64_t k = d >= 0 ? d / s : -((-d + s - 1) / s), off = d - k * s;      // row i of b begins `off` behind row i + k of a
+    return (k > -rows && k < rows && off < w) || (k + 1 > -rows && k + 1 < rows && s - off < w);
+  }
+  for (int64_t i = 0, j = 0; i < rows && j < rows;) {      // both ascend
+    const int64_t x = i * s, y = d + j * t;
+    if (x < y + w && y < x + w) return true;
+    if (x < y) ++i;
+    else ++j;
+  }
+  return false;
+}
+int check_gradient(const char *who, const wd_seq_rows_t &q, const void *dlogits, int64_t ld) {
+  const int64_t size = q.dtype == WD_T_F32 ? 4 : 2;
+  if (!dlogits) return WD_OK;
+  if (ld < q.vocab) { set_error("%s: row stride of the gradient below the row length", who); return WD_ERR_INVALID; }
+  if ((uintptr_t)dlogits % size) { set_error("%s: gradient not aligned to its element size", who); return WD_ERR_INVALID; }
+  if (meet(q.logits, q.ld * size, dlogits, ld * size, q.rows, q.vocab * size)) { set_error("%s: the gradient shares memory with the logits without being in their place", who); return WD_ERR_INVALID; }
+  return WD_OK;
+}
+
 int words(const wd_seq_rows_t &q) { return (int)(q.vocab / (q.dtype == WD_T_F32 ? 4 : 8)); }      // whole words of a row, at most
 
 // parts of a row: two workgroups for every CU where there are few rows, at least 4 KB each; a power of two up to a wavefront of them
@@ -1281,8 +1307,7 @@ extern "C" int wd_pref_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_pref_t *
   WD_REQUIRE(o.label_smoothing >= 0.f && o.label_smoothing < 0.5f, "label_smoothing must be in [0, 0.5)");
   WD_REQUIRE(o.kind == WD_PREF_LOGISTIC || (o.label_smoothing == 0.f && o.margin == 0.f), "label_smoothing and margin belong to the logistic loss");
   WD_REQUIRE(o.loss && (q.nseq == 0 || (o.pair_loss && o.difference && o.seq_logp)) && (q.rows == 0 || o.token_logp), "null output");
-  WD_REQUIRE(!o.dlogits || o.ld_dlogits >= q.vocab, "row stride of the gradient below the row length");
-  WD_REQUIRE((uintptr_t)o.dlogits % (q.dtype == WD_T_F32 ? 4 : 2) == 0, "gradient not aligned to its element size");
+  if (const int rc = check_gradient(__func__, q, o.dlogits, o.ld_dlogits)) return rc;
   hipStream_t st = as_stream(stream);
   const Work k(q, ws);
   const int ns = row_split(q);
@@ -1313,8 +1338,7 @@ extern "C" int wd_policy_loss_fwd_bwd(const wd_seq_rows_t *rows, const wd_policy
   WD_REQUIRE(o.clip_low >= 0.f && o.clip_low <= 1.f && o.clip_high >= 0.f, "clip range: low in [0, 1], high >= 0");
   WD_REQUIRE(o.kl_coef == 0.f || o.ref_logp || q.rows == 0, "a KL term needs the reference policy's log-probabilities");
   WD_REQUIRE(o.sums && (q.rows == 0 || (o.old_logp && o.token_logp)) && (o.advantages || (o.adv_per_row ? q.rows : q.nseq) == 0), "null pointer");
-  WD_REQUIRE(!o.dlogits || o.ld_dlogits >= q.vocab, "row stride of the gradient below the row length");
-  WD_REQUIRE((uintptr_t)o.dlogits % (q.dtype == WD_T_F32 ? 4 : 2) == 0, "gradient not aligned to its element size");
+  if (const int rc = check_gradient(__func__, q, o.dlogits, o.ld_dlogits)) return rc;
   hipStream_t st = as_stream(stream);
   if (tiny(q)) {
     by_type(q.dtype, [&](auto dt) { k_policy_tiny<decltype(dt)::value><<<tiny_grid(q, o.dlogits, o.ld_dlogits), 1024, 0, st>>>(q, o); });
