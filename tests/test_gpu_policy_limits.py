@@ -148,3 +148,29 @@ def test_gradients_beside_the_logits_rows():
                 with pytest.raises(capi.WdError, match="shares memory"):
                     call(bad)
             assert torch.equal(z, was)
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", SHAPES + [(1, 7, "f16"), (64, 1000, "bf16"), (1024, 64, "f32"), (5, 70001, "f32")])
+def test_losses_without_a_gradient(rows, vocab, dtype):
+    """dlogits None: the same bits as beside a gradient, and nothing else is written."""
+    from wide_deep_amd import policy
+    g = torch.Generator("cuda").manual_seed(rows)
+    z = torch.randn(rows, vocab, device="cuda", generator=g).to(DTYPES[dtype])
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    t[rows // 3] = -1
+    cuts = sorted({0, rows // 5, rows // 2, rows // 2 + 1, rows} & set(range(rows + 1)))
+    offs = torch.tensor(cuts + [rows] * (5 - len(cuts)), dtype=torch.int32, device="cuda")
+    was = z.clone()
+    ref = torch.randn(4, device="cuda", generator=g)
+    for kw in (dict(), dict(kind="square", length_norm=True, reduction="mean"), dict(margin=0.3, label_smoothing=0.1, weights=torch.rand(2, device="cuda", generator=g))):
+        full = policy.preference_loss(z, t, offs, ref_logp=ref, **kw)
+        for none in (None, False):
+            alone = policy.preference_loss(z, t, offs, ref_logp=ref, dlogits=none, **kw)
+            assert alone.dlogits is None and all(torch.equal(x, y) for x, y in zip(alone[:5], full[:5])) and bool(full.loss.isfinite())
+    old = policy.sequence_logp(z, t, offs).token_logp + torch.randn(rows, device="cuda", generator=g) * 0.1
+    adv = torch.randn(4, device="cuda", generator=g)
+    for kw in (dict(reduction="sum"), dict(reduction="token_mean", ref_logp=old, kl_coef=0.1), dict(reduction="sequence_mean")):
+        full = policy.policy_loss(z, t, offs, old, adv, per_row=False, **kw)
+        alone = policy.policy_loss(z, t, offs, old, adv, per_row=False, dlogits=None, **kw)
+        assert alone.dlogits is None and all(torch.equal(x, y) for x, y in zip(alone[:4], full[:4])) and bool(full.loss.isfinite())
+    assert torch.equal(z, was)
