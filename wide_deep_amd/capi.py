@@ -318,7 +318,7 @@ def load():
     lib.wd_last_error.restype = ctypes.c_char_p
     lib.wd_last_error.argtypes = []
     if "WD_HIP_LIB" not in os.environ:
-        # the prebuilt library ships with the tree (gpurun copies it): it must have been built from THESE sources
+        # a prebuilt library ships with the tree: it must have been built from THESE sources
         want = source_stamp()
         try:
             lib.wd_build_stamp.restype = ctypes.c_char_p

@@ -124,7 +124,7 @@ template <int N> __device__ __forceinline__ void hold(u32x4 (&w)[N]) {
   for (int u = 0; u < N; ++u) asm volatile("" : "+v"(w[u]));
 }
 template <int DT> __device__ __forceinline__ void store_word(typename Elem<DT>::type *g, bool aligned, const float *x) {
-  if (aligned) {      // the gradient is not read here: it need not push the logits out of the last cache (policy, odd catalogue: 48 -> 36 us)
+  if (aligned) {      // the gradient is not read here: it need not push the logits out of the last cache (policy loss of 988 x 50021 fp16: 48 -> 36 us)
     __builtin_nontemporal_store(Elem<DT>::pack(x), (u32x4 *)g);
     return;
   }
@@ -142,7 +142,7 @@ __device__ __forceinline__ void join(float &m, float &s, float m2, float s2) {
 }
 
 // Reductions of a wavefront, the same value in every lane.  Neighbours meet inside their row of 16 lanes (each quad holds one value after the
-// first two steps, so a mirrored row is an exchange), rows by the swaps of rows and halves: no trip through LDS, 6 steps of a few cycles each (policy, odd catalogue 35.5 -> 34.3 us).
+// first two steps, so a mirrored row is an exchange), rows by the swaps of rows and halves: no trip through LDS, 6 steps of a few cycles each (policy loss of 988 x 50021 fp16 35.5 -> 34.3 us).
 template <typename T, typename F> __device__ __forceinline__ T by_words(T v, F f) {
   static_assert(sizeof(T) == 4 || sizeof(T) == 8, "words");
   if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, f(__builtin_bit_cast(uint32_t, v)));

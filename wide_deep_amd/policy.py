@@ -3,11 +3,13 @@
 The reference knows one head, the sigmoid cross entropy of a click (wd_bce_sum_fwd_bwd); these stand beside it for models whose logits
 are a row of scores per position.  Each call is one entry of the C ABI (include/wd_hip.h, csrc/policy_loss.hip): loss AND gradient of
 the logits, launched on the current stream of the logits' device, nothing read back, so every call can be captured into a hipGraph.
-There is no autograd in between: `dlogits` goes to the backward pass of whatever made the logits (wd_gemm_*, the engine's towers).
+There is no autograd in between: `dlogits` goes to the backward pass of whatever made the logits, a program's own (wd_gemm_*, torch.mm).
+The engine's towers are no such producer: they make their gradient from the click loss inside the step and take none from outside.
 
 Layout of a batch: `logits` [rows, vocab] (fp32, fp16 or bf16; rows may be strided, items contiguous), `targets` int32 [rows] (outside
 [0, vocab), e.g. -1: the position is no action of the policy), `seq_offs` int32 [sequences + 1], a CSR over the rows.  Results and
-workspace come from torch's caching allocator on the current stream: calls on several streams share nothing.  Every tensor has to be
+workspace come from torch's caching allocator on the current stream: calls on several streams share nothing.  The results of a call but for
+`dlogits` are parts of one allocation with its workspace (11 floats a row, up to 2048 more where few rows are split): clone what is kept long.  Every tensor has to be
 ready on the current stream; one that another stream uses later is the caller's to record there.
 """
 import functools
